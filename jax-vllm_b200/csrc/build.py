@@ -30,7 +30,8 @@ ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--shared", "-Xcompiler", "-fPIC"]
 HEADERS = sorted(p.name for p in SRC_DIR.glob("*.cuh"))     # every shared header counts for every hash
 # further files that a source includes (they count for its hash)
-DEPENDS = {"attn_decode_static": ["attn_mma.cu", "attn_decode_static.h"]}
+DEPENDS = {"attn_decode_static": ["attn_mma.cu", "attn_decode_static.h"], "sampling": ["sampling.h"],
+           "sample_filtered": ["sampling.h", "vocab_row.h"], "token_logprobs": ["vocab_row.h"]}
 
 _loaded: dict[str, ctypes.CDLL] = {}
 _lock = threading.Lock()

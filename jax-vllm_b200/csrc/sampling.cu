@@ -5,42 +5,7 @@
 //       counter-based generator keyed by (seed of the request, index of the output token,
 //       v).  The draw therefore depends on the request and the place in its output only,
 //       not on the batch it was sampled in.
-#include "common.cuh"
-#include <math.h>
-
-__host__ __device__ __forceinline__ unsigned long long jv_mix64(unsigned long long z) {
-  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ULL;
-  z = (z ^ (z >> 27)) * 0x94D049BB133111EBULL;
-  return z ^ (z >> 31);
-}
-
-// Uniform in (0, 1) with 24 random bits.
-__host__ __device__ __forceinline__ float jv_uniform(unsigned long long seed, unsigned long long counter,
-                                                     unsigned long long v) {
-  unsigned long long h = jv_mix64(seed + 0x9E3779B97F4A7C15ULL * (counter + 1));
-  h = jv_mix64(h ^ (v * 0xD1342543DE82EF95ULL + 0x2545F4914F6CDD1DULL));
-  return ((float)(unsigned)(h >> 40) + 0.5f) * (1.0f / 16777216.0f);
-}
-
-// (value, index) ordering: larger value wins, the lower index among equal values.
-__device__ __forceinline__ void take_better(float& bv, int& bi, float ov, int oi) {
-  if (ov > bv || (ov == bv && oi < bi)) { bv = ov; bi = oi; }
-}
-
-__device__ __forceinline__ void block_best(float& bv, int& bi, float* sv, int* si) {
-  for (int o = 16; o > 0; o >>= 1)
-    take_better(bv, bi, __shfl_xor_sync(0xffffffffu, bv, o), __shfl_xor_sync(0xffffffffu, bi, o));
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (lane == 0) { sv[warp] = bv; si[warp] = bi; }
-  __syncthreads();
-  if (warp == 0) {
-    const int nwarps = blockDim.x >> 5;
-    bv = lane < nwarps ? sv[lane] : -INFINITY;
-    bi = lane < nwarps ? si[lane] : 0x7fffffff;
-    for (int o = 16; o > 0; o >>= 1)
-      take_better(bv, bi, __shfl_xor_sync(0xffffffffu, bv, o), __shfl_xor_sync(0xffffffffu, bi, o));
-  }
-}
+#include "sampling.h"
 
 // Stage 1: block (chunk, row) finds the best entry of its part of the vocabulary.
 __global__ void sample_partial_kernel(const float* __restrict__ logits, int vocab, int chunk,

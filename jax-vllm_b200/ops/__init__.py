@@ -13,8 +13,11 @@ kernel of this package.
 from __future__ import annotations
 
 import ctypes
+import math
+import operator
 import os
-from ctypes import c_float, c_int, c_longlong, c_void_p
+import struct
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 
 import torch
 
@@ -2526,3 +2529,207 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, seeds: torch.Tensor,
     _check(f(logits.data_ptr(), rows, vocab, temperature.data_ptr(), seeds.data_ptr(), counters.data_ptr(),
              part_v.data_ptr(), part_i.data_ptr(), out.data_ptr(), _stream()), "sample", launches=2)
     return out
+
+
+_SAMPLE_FILTERED_TYPES = [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                          c_void_p]
+_TOKEN_LOGPROBS_TYPES = [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+MOST_VOCAB = 1 << 20               # tokens of a row that `sample_filtered` and `token_logprobs` take
+MOST_TOP = 128                     # likeliest tokens a row that `token_logprobs` gives
+
+
+def _logit_rows(who: str, logits: torch.Tensor, values) -> tuple:
+    """(rows, vocab, elements between rows) of a matrix of logits whose rows are contiguous; `values`: (name, tensor, dtype)
+    of what stands beside them, one number a row."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
+        raise KernelError(f"{who}: logits are a matrix [rows, vocab]")
+    rows, vocab = logits.shape
+    if vocab < 1 or vocab > MOST_VOCAB:
+        raise KernelError(f"{who}: rows of 1 to {MOST_VOCAB} logits, got {vocab}")
+    if logits.dtype not in DTYPE_CODE:
+        raise KernelError(f"{who}: logits must be float32 or bfloat16, got {logits.dtype}")
+    stride = logits.stride(0) if rows > 1 else vocab
+    if (vocab > 1 and logits.stride(1) != 1) or stride < vocab:
+        raise KernelError(f"{who}: the logits of a row must be contiguous, and rows must not overlap")
+    for name, t, dtype in values:
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous():
+            raise KernelError(f"{who}: {name} must be {dtype}, contiguous, one value for each of the {rows} rows")
+        if t.device != logits.device:
+            raise KernelError(f"{who}: {name} is on {t.device}, the logits on {logits.device}")
+    _on_current_device(who, logits)
+    return rows, vocab, stride
+
+
+def _on_current_device(who: str, t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise KernelError(f"{who}: the tensors must be CUDA tensors (this engine has no CPU path)")
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"{who}: the tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
+                    seeds: torch.Tensor, counters: torch.Tensor) -> torch.Tensor:
+    """One token (int32) per row of float32 or bfloat16 logits, drawn from softmax(logits / temperature) over what the row's
+    filters leave.  With the tokens in order of their logits (the lowest index first among equal ones) and
+    p = exp((logit - largest) / temperature):
+
+        top_k > 0 (int32)    the first top_k tokens
+        min_p > 0            of these, the ones with p >= min_p (more than 1 counts as 1)
+        top_p < 1            of these, the ones before which less than top_p of their sum of p lies; the first always
+
+    The draw is the kept token with the largest logit / temperature - log(-log(u)), where u depends on (seed, counter,
+    token id) only: the numbers of `sample`, whose tokens a row without filters gets.  A temperature of 0 takes the largest
+    logit.  A NaN counts as minus infinity; a row with nothing else gives token 0."""
+    rows, vocab, stride = _logit_rows("sample_filtered", logits, (
+        ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+        ("min_p", min_p, torch.float32), ("seeds", seeds, torch.int64), ("counters", counters, torch.int64)))
+    out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    if rows == 0:
+        return out
+    f = _fn("sample_filtered", "jv_sample_filtered", _SAMPLE_FILTERED_TYPES)
+    _check(f(logits.data_ptr(), DTYPE_CODE[logits.dtype], stride, rows, vocab, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
+             min_p.data_ptr(), seeds.data_ptr(), counters.data_ptr(), out.data_ptr(), _stream()), "sample_filtered")
+    return out
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> tuple:
+    """(logprob [rows], top_tokens [rows, top], top_logprobs [rows, top]): log softmax(logits) at one token (int32) per row of
+    float32 or bfloat16 logits, and the `top` likeliest tokens (at most 128) with theirs, equal ones in the order of their
+    indices.  32-bit.  A NaN counts as minus infinity; in a row with nothing else every logprob is minus infinity.  A token
+    outside the vocabulary sets the status word and gives NaN."""
+    rows, vocab, stride = _logit_rows("token_logprobs", logits, (("tokens", tokens, torch.int32),))
+    top = int(top)
+    if top < 0 or top > MOST_TOP or top > vocab:
+        raise KernelError(f"token_logprobs: top must be 0 to {min(MOST_TOP, vocab)}, got {top}")
+    device = logits.device
+    logprob = torch.empty(rows, dtype=torch.float32, device=device)
+    top_tokens = torch.empty((rows, top), dtype=torch.int32, device=device)
+    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
+    if rows == 0:
+        return logprob, top_tokens, top_logprobs
+    f = _fn("token_logprobs", "jv_token_logprobs", _TOKEN_LOGPROBS_TYPES)
+    _check(f(logits.data_ptr(), DTYPE_CODE[logits.dtype], stride, rows, vocab, tokens.data_ptr(), top, logprob.data_ptr(),
+             top_tokens.data_ptr(), top_logprobs.data_ptr(), _status_ptr(device), _stream()), "token_logprobs")
+    return logprob, top_tokens, top_logprobs
+
+
+# ------------------------------------------------------------------- copies inside a cache
+def _index_list(who: str, name: str, ids) -> list:
+    """`ids` as a list of ints: indices that the host knows (a launch carries them as parameters)."""
+    if isinstance(ids, torch.Tensor):
+        if ids.is_cuda or ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64):
+            raise KernelError(f"{who}: {name} must be integers on the host")
+        return ids.tolist()
+    ids = list(ids)
+    if not all(type(i) is int for i in ids):
+        try:
+            ids = [operator.index(i) for i in ids]
+        except TypeError:
+            raise KernelError(f"{who}: {name} must be integers") from None
+    return ids
+
+
+def check_copies(who: str, src, dst, n_src: int, n_dst: int, apart: bool, tokens=None, most: int = 0) -> tuple:
+    """(src, dst, tokens) as lists, after the checks of a copy: indices that exist, no destination twice and, unless sources
+    and destinations are `apart`, none that is a source too."""
+    src, dst = _index_list(who, "src", src), _index_list(who, "dst", dst)
+    if len(src) != len(dst):
+        raise KernelError(f"{who}: {len(src)} sources and {len(dst)} destinations")
+    if tokens is not None:
+        tokens = _index_list(who, "tokens", tokens)
+        if len(tokens) != len(src):
+            raise KernelError(f"{who}: one number of tokens per pair")
+        if tokens and (min(tokens) < 0 or max(tokens) > most):
+            raise KernelError(f"{who}: a page holds 0 to {most} tokens")
+    if not src:
+        return src, dst, tokens
+    if min(src) < 0 or max(src) >= n_src or min(dst) < 0 or max(dst) >= n_dst:
+        raise KernelError(f"{who}: sources lie in [0, {n_src}), destinations in [0, {n_dst})")
+    written = set(dst)
+    if len(written) != len(dst):
+        raise KernelError(f"{who}: a destination is given twice")
+    if not apart and not written.isdisjoint(src):
+        raise KernelError(f"{who}: a destination is a source too")
+    return src, dst, tokens
+
+
+def _span(t: torch.Tensor) -> tuple:
+    """First byte and one past the last of what a tensor's elements cover."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _copy_planes(who: str, planes: list, src: list, dst: list, tokens) -> None:
+    """planes: nine numbers each, as csrc/page_copy.cu takes them."""
+    n = len(src)
+    pairs = [0] * (3 * n)
+    pairs[0::3], pairs[1::3], pairs[2::3] = src, dst, tokens if tokens is not None else [-1] * n
+    flat = [v for plane in planes for v in plane]
+    launches = -(-len(planes) // 64) * -(-n // 1024)
+    f = _fn("page_copy", "jv_page_copy", [c_char_p, c_int, c_char_p, c_int, c_void_p])
+    _check(f(struct.pack(f"{len(flat)}q", *flat), len(planes), struct.pack(f"{3 * n}i", *pairs), n, _stream()), who, launches=launches)
+
+
+def copy_pages(stores, src, dst, tokens=None, into=None) -> None:
+    """Copies pages of a cache: page src[i] of every store [layers, pages, page_size, ...] to page dst[i] of the same store, or
+    of the store at the same place of `into` (a pool of another size).  src and dst are integers on the host; no page is
+    given twice as a destination, and in place none is both source and destination.  `tokens[i]` copies only the first
+    so many tokens of the page; what follows them in the destination stays as it was.  A store may have any strides over
+    layers and pages; a page itself is contiguous.  The stores of `into` lie apart in memory from those that are read."""
+    stores = list(stores)
+    to = stores if into is None else list(into)
+    if not stores or len(to) != len(stores):
+        raise KernelError("copy_pages: a list of stores, and as many to copy into")
+    for a, b in zip(stores, to):
+        if not isinstance(a, torch.Tensor) or not isinstance(b, torch.Tensor) or a.dim() < 3 or a.shape[:1] + a.shape[2:] != b.shape[:1] + b.shape[2:] \
+                or a.dtype != b.dtype or a.device != b.device:
+            raise KernelError("copy_pages: stores are [layers, pages, page_size, ...]; what is copied into has the same type, device and shape but for the pages")
+        if a.shape[1:3] != stores[0].shape[1:3] or b.shape[1] != to[0].shape[1]:
+            raise KernelError("copy_pages: all stores have the same number of pages and of tokens in a page")
+    src, dst, tokens = check_copies("copy_pages", src, dst, stores[0].shape[1], to[0].shape[1], into is not None, tokens, stores[0].shape[2])
+    planes = []
+    for a, b in zip(stores, to):
+        _on_current_device("copy_pages", a)
+        page = math.prod(a.shape[2:])
+        for t in (a, b):
+            if t.numel() and not t[0, 0].is_contiguous():
+                raise KernelError("copy_pages: a page must be contiguous")
+            (n0, n1), (s0, s1) = t.shape[:2], t.stride()[:2]
+            if t.numel() and not (n0 == 1 or s0 >= (n1 - 1) * s1 + page) and not (n1 == 1 or s1 >= (n0 - 1) * s0 + page) \
+                    or (n0 > 1 and s0 < page) or (n1 > 1 and s1 < page):
+                raise KernelError("copy_pages: pages must not overlap")
+        size = a.element_size()
+        planes.append((a.data_ptr(), b.data_ptr(), a.stride(0) * size, a.stride(1) * size, b.stride(0) * size, b.stride(1) * size,
+                       page * size, page // max(1, a.shape[2]) * size, a.shape[0]))
+    if into is not None:
+        spans = [_span(t) for t in to if t.numel()]
+        for x in (_span(t) for t in stores if t.numel()):
+            if any(x[0] < y[1] and y[0] < x[1] for y in spans):
+                raise KernelError("copy_pages: the stores to copy into must lie apart from the others in memory")
+    if src and all(p[6] and p[8] for p in planes):
+        _copy_planes("copy_pages", planes, src, dst, tokens)
+
+
+def copy_slots(states, src, dst) -> None:
+    """Copies rows of per-request state: row src[i] of every tensor [slots, ...] to row dst[i] of the same tensor, under the
+    rules of `copy_pages`.  The tensors may have different shapes behind the slots, and different types."""
+    states = list(states)
+    if not states:
+        raise KernelError("copy_slots: a list of state tensors")
+    slots = states[0].shape[0] if isinstance(states[0], torch.Tensor) and states[0].dim() else 0
+    src, dst, _ = check_copies("copy_slots", src, dst, slots, slots, False)
+    planes = []
+    for t in states:
+        if not isinstance(t, torch.Tensor) or t.dim() < 1 or t.shape[0] != slots:
+            raise KernelError("copy_slots: all states are [slots, ...] with the same number of slots")
+        _on_current_device("copy_slots", t)
+        row = math.prod(t.shape[1:])
+        if t.numel() and not t[0].is_contiguous():
+            raise KernelError("copy_slots: a row must be contiguous")
+        if slots > 1 and t.stride(0) < row:
+            raise KernelError("copy_slots: rows must not overlap")
+        size = t.element_size()
+        if row:
+            planes.append((t.data_ptr(), t.data_ptr(), 0, t.stride(0) * size, 0, t.stride(0) * size, row * size, row * size, 1))
+    if src and planes:
+        _copy_planes("copy_slots", planes, src, dst, None)
