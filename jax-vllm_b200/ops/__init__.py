@@ -2531,9 +2531,9 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, seeds: torch.Tensor,
     return out
 
 
-_SAMPLE_FILTERED_TYPES = [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+_SAMPLE_FILTERED_TYPES = [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                           c_void_p]
-_TOKEN_LOGPROBS_TYPES = [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+_TOKEN_LOGPROBS_TYPES = [c_void_p, c_int, c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]
 MOST_VOCAB = 1 << 20               # tokens of a row that `sample_filtered` and `token_logprobs` take
 MOST_TOP = 128                     # likeliest tokens a row that `token_logprobs` gives
 
@@ -2588,7 +2588,7 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
         return out
     f = _fn("sample_filtered", "jv_sample_filtered", _SAMPLE_FILTERED_TYPES)
     _check(f(logits.data_ptr(), DTYPE_CODE[logits.dtype], stride, rows, vocab, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
-             min_p.data_ptr(), seeds.data_ptr(), counters.data_ptr(), out.data_ptr(), _stream()), "sample_filtered")
+             min_p.data_ptr(), seeds.data_ptr(), counters.data_ptr(), out.data_ptr(), 0, _stream()), "sample_filtered")
     return out
 
 
@@ -2609,7 +2609,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         return logprob, top_tokens, top_logprobs
     f = _fn("token_logprobs", "jv_token_logprobs", _TOKEN_LOGPROBS_TYPES)
     _check(f(logits.data_ptr(), DTYPE_CODE[logits.dtype], stride, rows, vocab, tokens.data_ptr(), top, logprob.data_ptr(),
-             top_tokens.data_ptr(), top_logprobs.data_ptr(), _status_ptr(device), _stream()), "token_logprobs")
+             top_tokens.data_ptr(), top_logprobs.data_ptr(), _status_ptr(device), 0, _stream()), "token_logprobs")
     return logprob, top_tokens, top_logprobs
 
 
