@@ -32,278 +32,337 @@ struct SampleParams {
 
 constexpr float DEEPEST = 30.f;
 constexpr int FIRST_LOOK = 128;                        // tokens that the list is meant to hold where no count says how many
+constexpr float LOG2E = 1.4426950408889634f;
 
 // The best score so far and its token.
 struct Best { float v; int i; };
 
 // Scores of one row: x / T - log(-log(u)) in the arithmetic of sampling.cu.
 struct Scores {
-  float temp, inv;
-  u64 seed, counter;
+  float temp, per;                                     // T and log2(e) / T
+  u64 base;
 
-  __device__ __forceinline__ float of(float x, int i) const {
-    return x / temp - logf(-logf(jv_uniform(seed, counter, (u64)i)));
+  __device__ __forceinline__ u64 bits(int i) const { return jv_draw_bits(base, (u64)i); }
+  __device__ __forceinline__ float of(float x, u64 bits) const {
+    return x / temp - logf(-logf(((float)(unsigned)(bits >> 40) + 0.5f) * (1.0f / 16777216.0f)));
   }
-  // A number that no score of x with the uniform number of token i is above, but for roundings: -log(-log(u)) <= -log(1 - u).
-  __device__ __forceinline__ float most(float x, int i) const {
-    const float w = 1.f - jv_uniform(seed, counter, (u64)i);
-    return fmaf(x, inv, -0.69314718f * __log2f(w));
+  // Whether the score may reach `enough` (given as enough * log2(e)), but for roundings: -log(-log(u)) <= -log(1 - u), and
+  // 1 - u is no less than what the first 23 random bits leave of it.
+  __device__ __forceinline__ bool may_reach(float x, u64 bits, float enough2) const {
+    const float w = (2.f - 1.1920929e-7f) - __uint_as_float(0x3f800000u | (unsigned)(bits >> 41));
+    return !(w > exp2_fast(fmaf(x, per, -enough2)));
   }
 };
 
-// The best score among the elements of this thread with c >= cut.  What a token can reach at most is compared with the best
-// score that the warp knows, less what the roundings of both may be (scores are off by a few 2^-24 of themselves, `most` by
-// a few more and by what the approximate logarithm lacks): few tokens need their logarithms.
-template <typename T>
-__device__ __forceinline__ void draw(const Reader<T>& rd, const Scores& sc, u64 cut, Best& best) {
-  const float low = logit_of(cut);
-  float enough = -INFINITY;
-  const int n = rd.n;
-  for_row<2, true>(rd.row, n, rd.me, rd.all, [&](const auto& x, int at) {
-    constexpr int V = sizeof(x) / sizeof(float);
-    bool better = false;
+// The best score of the tokens that it is called for, a vector at a time and by whole warps.  What a token can reach at most is
+// compared with the best score that the block knows (which a warp may see late: it only saves work), less what the roundings
+// of both may be (scores are off by a few 2^-24 of themselves, the bound by a few more and by what the approximate exponential
+// lacks): few tokens need their logarithms.
+struct Draw {
+  const Scores sc;
+  Best best{-INFINITY, 0x7fffffff};
+  float enough2 = -INFINITY;
+
+  __device__ __forceinline__ Draw(const Scores& sc_) : sc(sc_) {}
+  // which: a bit for each value that is drawn from
+  template <int VEC> __device__ __forceinline__ void operator()(const float (&x)[VEC], int at, unsigned which) {
+    if (!__any_sync(0xffffffffu, which != 0)) return;
+    unsigned may = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float y = clean(x[i]);
-      if (y >= low && at + i < n && !(sc.most(y, at + i) < enough) && compose(y, at + i) >= cut) {
-        const float v = best.v;
-        take_better(best.v, best.i, sc.of(y, at + i), at + i);
-        better |= best.v > v;
-      }
+    for (int i = 0; i < VEC; ++i) may |= sc.may_reach(x[i], sc.bits(at + i), enough2) ? 1u << i : 0u;
+    may &= which;
+    for (unsigned left = __reduce_or_sync(0xffffffffu, may); left; left &= left - 1) {
+      const int i = __ffs(left) - 1;
+      float y = x[0];
+#pragma unroll
+      for (int k = 1; k < VEC; ++k) y = i == k ? x[k] : y;
+      const u64 bits = sc.bits(at + i);
+      const bool still = (may >> i & 1) && sc.may_reach(y, bits, enough2);
+      if (!__any_sync(0xffffffffu, still)) continue;
+      if (still) take_better(best.v, best.i, sc.of(y, bits), at + i);
+      const unsigned known = __reduce_max_sync(0xffffffffu, key_of(best.v));
+      unsigned of_block = known;
+      if ((threadIdx.x & 31) == 0) of_block = max(known, atomicMax(&shared().best_key, known));
+      const float enough = value_of(__shfl_sync(0xffffffffu, of_block, 0));
+      enough2 = (enough - (1e-5f * fabsf(enough) + 1e-3f)) * LOG2E;
     }
-    if constexpr (V > 1) {
-      if (__any_sync(0xffffffffu, better)) {
-        const float known = value_of(__reduce_max_sync(0xffffffffu, key_of(best.v)));
-        enough = known - (1e-5f * fabsf(known) + 1e-3f);
-      }
+  }
+};
+
+// The best score of the tokens with c >= cut.
+template <typename T> __device__ __noinline__ Best draw_from(const Scores sc, u64 cut) {
+  Draw draw(sc);
+  const float lowest = logit_of(cut);
+  const bool ragged = (cut & (MAX_VOCAB - 1)) != 0;    // they begin among equal logits
+  each<T, 2, true>([&](const auto& x, int at) {
+    unsigned which = 0;
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) which |= x[i] >= lowest ? 1u << i : 0u;
+    if (ragged) {
+#pragma unroll
+      for (int i = 0; i < 16 / (int)sizeof(T); ++i)
+        if (x[i] == lowest && compose(clean(x[i]), at + i) < cut) which &= ~(1u << i);
+    }
+    draw(x, at, which);
+  });
+  return draw.best;
+}
+// Puts the tokens of the range and, with `score`, gives the best score of those above it.
+template <typename T> __device__ __noinline__ Best draw_above(const Scores sc, u64 cut, bool score) {
+  Draw draw(sc);
+  put_range<T, true, true>(cut, [&](const auto& x, int at, unsigned which) { if (score) draw(x, at, which); });
+  return draw.best;
+}
+template <typename T> __device__ __noinline__ Best largest_of_row() {
+  Best best{-INFINITY, 0x7fffffff};
+  each<T, 8>([&](const auto& x, int at) {
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i)
+      if (x[i] > best.v) best = Best{x[i], at + i};    // a thread's tokens come in the order of their indices
+  });
+  return best;
+}
+
+// The second pass of a row whose first tokens a list may hold: puts those at or above `least` in it.  SUMMED: returns the masses
+// of the tokens from `low` up, and of those that are put.
+template <typename T, bool SUMMED> __device__ __noinline__ float2 list_first(float low, float least) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const float largest = shared().largest, scale = shared().scale;
+  float all = 0.f, listed = 0.f;
+  each<T, 4>([&](const auto& x, int at) {
+    float big = x[0];                                  // (a NaN is passed over)
+#pragma unroll
+    for (int i = 1; i < VEC; ++i) big = fmaxf(big, x[i]);
+    if (SUMMED) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) all += x[i] >= low ? exp2_fast(-(below(x[i], largest) * scale)) : 0.f;
+    }
+    if (big >= least) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (x[i] >= least) {
+          if (SUMMED) listed += exp2_fast(-(below(x[i], largest) * scale));
+          put(compose(clean(x[i]), at + i));
+        }
     }
   });
+  return make_float2(all, listed);
 }
 
-// Prefix sums over the first block of the masses of the list's first `listed` tokens, two a thread: before[j] lies before
-// the token 2 * threadIdx.x + j.  Returns the sum of all.
-__device__ __forceinline__ double masses_before(Shared& sh, int listed, float largest, float scale, double (&before)[2]) {
+// First block only: the mass of the list's first m tokens, and how many of them have less than `part` of the mass that counts
+// before them (with `above` before the first): `mass`, or the list's where that is negative.
+static __device__ __noinline__ int kept_by_mass(int m, double above, double part, double mass, double& sum) {
+  constexpr int PER = LIST / NT;
+  Shared& sh = shared();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  double q[2];
+  const float largest = sh.largest, scale = sh.scale;
+  double q[PER], s = 0.;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int i = 2 * threadIdx.x + j;
-    q[j] = i < listed ? (double)mass_of(logit_of(sh.list[i]), largest, scale) : 0.;
+  for (int j = 0; j < PER; ++j) {
+    const int i = PER * threadIdx.x + j;
+    q[j] = i < m ? (double)exp2_fast(-(below(logit_of(sh.list[i]), largest) * scale)) : 0.;
+    s += q[j];
   }
-  double s = q[0] + q[1];
+  double to = s;
   for (int o = 1; o < 32; o *= 2) {
-    const double t = __shfl_up_sync(0xffffffffu, s, o);
-    if (lane >= o) s += t;
+    const double t = __shfl_up_sync(0xffffffffu, to, o);
+    if (lane >= o) to += t;
   }
-  double own = __shfl_up_sync(0xffffffffu, s, 1);
-  if (lane == 0) own = 0.;
   __syncthreads();
-  if (lane == 31) sh.warp_d[0][warp] = s;
+  if (lane == 31) sh.warp_d[0][warp] = to;
   __syncthreads();
-  double base = 0., total = 0.;
+  double before = above, total = 0.;
   for (int w = 0; w < WARPS; ++w) {
-    if (w == warp) base = total;
+    if (w < warp) before += sh.warp_d[0][w];
     total += sh.warp_d[0][w];
   }
-  before[0] = base + own;
-  before[1] = before[0] + q[0];
-  return total;
+  sum = total;
+  const double first = __shfl_up_sync(0xffffffffu, to, 1), end = part * (mass < 0. ? total : mass);
+  if (lane > 0) before += first;
+  int mine = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = PER * threadIdx.x + j;
+    if (i < m && (before == 0. || before < end)) mine = i + 1;
+    before += q[j];
+  }
+  mine = __reduce_max_sync(0xffffffffu, mine);
+  if (lane == 0) sh.warp_i[warp] = mine;
+  __syncthreads();
+  int kept = 0;
+  for (int w = 0; w < WARPS; ++w) kept = max(kept, sh.warp_i[w]);
+  __syncthreads();
+  return kept;
 }
 
-static_assert(LIST == 2 * NT, "two tokens of the list a thread");
+// A row with filters.  Returns the first token number that is kept where all tokens from there on are still to be drawn from;
+// 0 where the first block has the others' best scores (with `drawn`) and `listed` kept tokens in its list; ~0 where nothing
+// is left to do for this block.
+template <typename T>
+__device__ __forceinline__ u64 filtered(const SampleParams& p, const Scores& sc, int top_k, float top_p, float min_p, Best& best, int& listed,
+                                        bool& drawn) {
+  Shared& sh = shared();
+  const float temp = sc.temp;
+  const bool by_count = top_k > 0 && top_k < p.vocab, by_mass = top_p < 1.f, by_share = min_p > 0.f;
+  // a list of the first tokens serves counts up to what the blocks' threads can bound
+  const int j = ((by_count ? top_k : min(FIRST_LOOK, FEW * p.blocks)) - 1) / p.blocks + 1;
+  const bool can_list = countable(j, p.blocks);
+  const bool summed = by_mass && !by_count;            // the mass that counts is that of the whole row
+  // one block a row: one pass, unless the mass that counts depends on the largest logit
+  const bool once = p.blocks == 1 && (by_count || by_mass) && can_list && !(summed && by_share);
+  if (threadIdx.x == 0) sh.scale = fminf(fmaxf(sc.per, 1e-37f), 3e38f);
+  float2 mine{-INFINITY, 0.f};
+  if (once) {
+    __syncthreads();
+    mine = summed ? put_once<T, true>(j, DEEPEST * temp) : put_once<T, false>(j, DEEPEST * temp);
+  } else {
+    mine.x = my_largest<T>();
+  }
+  started();
+  exchange_largest(mine.x, can_list ? j : FEW);
+  const float largest = sh.largest;
+  if (largest == -INFINITY) return ~0ull;              // nothing is left in the row (the output says 0 already)
+  // the lowest logit that any filter may keep
+  float low = largest - DEEPEST * temp;
+  if (!(low <= largest)) low = largest;                // (infinite numbers that make none)
+  if (by_share) {
+    const double least = (double)largest + (double)temp * log((double)fminf(min_p, 1.f));
+    if (!(least <= (double)largest)) low = largest;
+    else low = fmaxf(low, __double2float_ru(least));
+  }
+  u64 cut = (u64)max(key_of(low + 0.f), KEY_LOWEST + 1) << INDEX_BITS;
+  if (!by_count && !by_mass) return cut;
+  low = logit_of(cut);
+
+  const float least = fmaxf(sh.bound, low);
+  unsigned total = LIST + 1;
+  bool found = false;
+  double mass = -1., list_mass = 0.;                   // mass: of what the count and the share leave, where it is known
+  if (once) {
+    total = keep_list(least);
+    found = total <= (unsigned)LIST;
+    if (found && summed) {
+      const double2 a = block_sums((double)(mine.x == largest ? mine.y : mine.y * exp2_fast(-(below(mine.x, largest) * sh.scale))), 0.);
+      if (threadIdx.x == 0) sh.part[0][0] = a.x;
+      __syncthreads();
+      mass = sh.part[0][0];
+    }
+  } else if (can_list && !(summed && largest - sh.bound < 3.f * temp)) {
+    // (of nearly even logits, those from the bound up would hold too little of the mass)
+    if (summed) {
+      const float2 q = list_first<T, true>(low, least);
+      const double2 a = block_sums((double)q.x, (double)q.y);
+      if (threadIdx.x == 0)
+        for (int b = 0; b < p.blocks; ++b) {
+          of(&sh.part[sh.rank][0], b)[0] = a.x;
+          of(&sh.part[sh.rank][0], b)[1] = a.y;
+        }
+    } else {
+      list_first<T, false>(low, least);
+    }
+    total = send_list();
+    found = total <= (unsigned)LIST;
+    if (summed) {
+      mass = 0.;
+      for (int b = 0; b < p.blocks; ++b) { mass += sh.part[b][0]; list_mass += sh.part[b][1]; }
+      found = found && (least == low || list_mass >= (double)top_p * mass);
+    }
+  }
+  if (found) {
+    if (sh.rank != 0) return ~0ull;
+    sort_list((int)total);
+    listed = by_count ? min(top_k, (int)total) : (int)total;
+    if (by_mass) listed = kept_by_mass(listed, 0., (double)top_p, mass, list_mass);
+    if (!(once && summed) || least == low || list_mass >= (double)top_p * mass) return 0;
+  }
+  if (threadIdx.x == 0) sh.listed = 0;
+
+  const float step = DEEPEST * temp, wide = 6.f * (largest - sh.bound);
+  const float per = (float)BINS / (wide > 0.f ? fminf(step, wide) : step);
+  if (by_count) {                                      // the boundary by count
+    if (!narrow<T, false>(cut, per, LIST / 2, (double)top_k, -1., (double)top_k)) {
+      if (!by_mass) return cut;                        // no more tokens than the count leaves
+    } else {
+      const double above = sh.range.above;
+      best = draw_above<T>(sc, cut, !by_mass);
+      total = send_list();
+      const bool last = !by_mass || above == 0.;
+      if (!by_mass) {
+        block_best(best.v, best.i, sh.warp_v, sh.warp_i);
+        if (threadIdx.x == 0) { *of(&sh.part_v[sh.rank], 0) = best.v; *of(&sh.part_i[sh.rank], 0) = best.i; }
+        sync_row();
+        drawn = true;
+      }
+      if (last && sh.rank != 0) return ~0ull;
+      if (sh.rank == 0) {
+        sort_list((int)total);
+        listed = top_k - (int)above;
+      }
+      if (last) {
+        if (by_mass) listed = kept_by_mass(listed, 0., (double)top_p, -1., list_mass);
+        return 0;
+      }
+      if (sh.rank == 0 && threadIdx.x == 0) sh.told = sh.list[listed - 1];
+      sync_row();
+      cut = *of(&sh.told, 0);
+      sync_row();                                      // it is read: the first block may go on to another one
+    }
+  }
+  narrow<T, true>(cut, per, LIST / 2, 0., (double)top_p, -1.);
+  best = draw_above<T>(sc, cut, true);
+  block_best(best.v, best.i, sh.warp_v, sh.warp_i);
+  if (threadIdx.x == 0) { *of(&sh.part_v[sh.rank], 0) = best.v; *of(&sh.part_i[sh.rank], 0) = best.i; }
+  total = send_list();
+  drawn = true;
+  if (sh.rank != 0) return ~0ull;
+  sort_list((int)total);
+  listed = kept_by_mass((int)total, sh.range.above, (double)top_p, sh.all, list_mass);
+  return 0;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(NT, 2) sample_filtered_kernel(const SampleParams p) {
-  extern __shared__ __align__(16) unsigned char memory[];
-  Shared& sh = *reinterpret_cast<Shared*>(memory);
+  Shared& sh = shared();
   pdl_trigger();
   pdl_wait();
   const int r = blockIdx.x / p.blocks;
-  Reader<T> rd;
-  rd.start(reinterpret_cast<const T*>(p.logits) + (size_t)r * p.stride, p.vocab, p.blocks, &sh);
+  begin(reinterpret_cast<const T*>(p.logits) + (size_t)r * p.stride, p.vocab, p.blocks);
   const float temp = p.temperature[r];
-  const bool hot = temp > 0.f;
   const int top_k = p.top_k[r];
   const float top_p = p.top_p[r], min_p = p.min_p[r];
-  const bool by_count = hot && top_k > 0 && top_k < p.vocab, by_mass = hot && top_p < 1.f, by_share = hot && min_p > 0.f;
-  const Scores sc{temp, 1.f / temp, (u64)p.seeds[r], (u64)p.counters[r]};
-
+  const Scores sc{temp, LOG2E / temp, jv_draw_base((u64)p.seeds[r], (u64)p.counters[r])};
+  if (sh.rank == 0 && threadIdx.x == 0) p.out[r] = 0;
   Best best{-INFINITY, 0x7fffffff};
-  bool in_list = false;                                // every kept token stands in the first block's list
   int listed = 0;                                      // first block: kept tokens of its sorted list
-
-  if (!hot) {
-    rd.template each<8>([&](const auto& x, int at) {
-      constexpr int V = sizeof(x) / sizeof(float);
-#pragma unroll
-      for (int i = 0; i < V; ++i) take_better(best.v, best.i, clean(x[i]), at + i);
-    });
-    rd.started();
-  } else if (!by_count && !by_mass && !by_share) {
-    draw(rd, sc, (u64)KEY_LOWEST << INDEX_BITS, best);
-    rd.started();
+  bool drawn = false;                                  // first block: it has the best scores of the tokens that are not listed
+  u64 cut = LOWEST;
+  const bool hot = temp > 0.f;
+  if (hot && ((top_k > 0 && top_k < p.vocab) || top_p < 1.f || min_p > 0.f)) {
+    cut = filtered<T>(p, sc, top_k, top_p, min_p, best, listed, drawn);
+    if (cut == ~0ull) return;
   } else {
-    // a list of the first tokens serves counts up to what the blocks' groups can bound
-    const int j = by_count ? (top_k - 1) / p.blocks + 1 : (FIRST_LOOK - 1) / p.blocks + 1;
-    const bool countable = j <= MOST_OF_GROUPS;
-    float m = -INFINITY;
-    rd.template each<8>([&](const auto& x, int) {
-      constexpr int V = sizeof(x) / sizeof(float);
-#pragma unroll
-      for (int i = 0; i < V; ++i) m = fmaxf(m, x[i]);
-    });
-    rd.started();
-    rd.exchange_largest(m, countable ? j : GROUPS / 2, [] {});
-    if (rd.largest == -INFINITY) {                     // nothing is left in the row
-      if (rd.rank == 0 && threadIdx.x == 0) p.out[r] = 0;
-      return;
-    }
-    rd.scale = 1.4426950408889634f * sc.inv;
-    // the lowest logit that any filter may keep
-    float low = rd.largest - DEEPEST * temp;
-    if (!(low <= rd.largest)) low = rd.largest;        // (infinite numbers that make none)
-    if (by_share) {
-      const double least = (double)rd.largest + (double)temp * log((double)fminf(min_p, 1.f));
-      if (!(least <= (double)rd.largest)) low = rd.largest;
-      else low = fmaxf(low, __double2float_ru(least));
-    }
-    u64 cut = (u64)max(key_of(low + 0.f), KEY_LOWEST + 1) << INDEX_BITS;
-    low = logit_of(cut);
-
-    if (by_count || by_mass) {
-      const auto bounded = [&](double q, double target) { return q == 0. || q < target; };
-      const bool summed = by_mass && !by_count;        // the mass that counts is that of the whole row
-      double mass_kept = 0.;
-      bool found = false;
-      if (countable) {
-        const float least = fmaxf(rd.bound, low);
-        float all_mass = 0.f, list_mass = 0.f;
-        rd.template each<4>([&](const auto& x, int at) {
-          constexpr int V = sizeof(x) / sizeof(float);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float y = x[i];                      // a NaN is no smaller than anything
-            float q = 0.f;
-            if (summed) {
-              q = y >= low ? mass_of(y, rd.largest, rd.scale) : 0.f;
-              all_mass += q;
-            }
-            if (y >= least) {
-              list_mass += q;
-              rd.put(compose(clean(y), at + i));
-            }
-          }
-        });
-        double a = all_mass, l = list_mass;
-        if (summed) rd.block_sums(a, l);
-        const unsigned total = rd.send_list([&] {
-          if (threadIdx.x == 0 && summed)
-            for (int b = 0; b < p.blocks; ++b) {
-              rd.of(&sh.part[rd.rank][0], b)[0] = a;
-              rd.of(&sh.part[rd.rank][0], b)[1] = l;
-            }
-        });
-        found = total <= (unsigned)LIST;
-        if (summed) {
-          l = 0.;
-          for (int b = 0; b < p.blocks; ++b) { mass_kept += sh.part[b][0]; l += sh.part[b][1]; }
-          found = found && (least == low || l >= (double)top_p * mass_kept);
-        }
-        if (found) {
-          if (rd.rank != 0) return;
-          in_list = true;
-          rd.sort_list((int)total);
-          listed = by_count ? min(top_k, (int)total) : (int)total;
-        } else if (threadIdx.x == 0) {
-          sh.listed = 0;
-        }
-      }
-      Range range{0, 0, 0., 0u, 0u};
-      if (!found) {
-        const float step = DEEPEST * temp, wide = 6.f * (rd.largest - rd.bound);
-        const float per = (float)BINS / (wide > 0.f ? fminf(step, wide) : step);
-        bool counted = false;
-        if (by_count) {
-          const auto whole = [&](unsigned n, double q) { mass_kept = q; return n > (unsigned)top_k; };
-          if (rd.template narrow<true>(cut, per, LIST, range, whole, [&](unsigned n, double) { return n < (unsigned)top_k; })) {
-            const unsigned total = rd.gather(range.lo, range.hi);
-            in_list = range.count_above == 0;
-            if (in_list && rd.rank != 0) return;
-            if (rd.rank == 0) {
-              rd.sort_list((int)total);
-              listed = top_k - (int)range.count_above;
-              double before[2];
-              const double q = masses_before(sh, listed, rd.largest, rd.scale, before);
-              if (threadIdx.x == 0) { sh.told = sh.list[listed - 1]; sh.told_mass = range.mass_above + q; }
-            }
-            if (!in_list) {
-              rd.sync();
-              cut = *rd.of(&sh.told, 0);
-              mass_kept = *rd.of(&sh.told_mass, 0);
-              rd.sync();                               // they are read: the first block may go on to other ones
-            }
-          }
-          counted = true;
-        }
-        if (by_mass && !in_list) {
-          double target = (double)top_p * mass_kept;
-          rd.template narrow<true>(cut, per, LIST, range, [&](unsigned, double q) {
-            if (!counted) { mass_kept = q; target = (double)top_p * q; }
-            return true;
-          }, [&](unsigned, double q) { return bounded(q, target); });
-          const unsigned total = rd.gather(range.lo, range.hi);
-          in_list = range.count_above == 0;
-          if (in_list && rd.rank != 0) return;
-          if (rd.rank == 0) {
-            rd.sort_list((int)total);
-            listed = (int)total;
-          }
-        }
-      }
-      if (by_mass && (rd.rank == 0 || !in_list)) {
-        if (rd.rank == 0) {
-          double before[2];
-          const double q = masses_before(sh, listed, rd.largest, rd.scale, before);
-          if (in_list && by_count) mass_kept = q;
-          const double target = (double)top_p * mass_kept, above = in_list ? 0. : range.mass_above;
-          int mine = 0;
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            if (2 * threadIdx.x + k < listed && bounded(above + before[k], target)) mine = 2 * threadIdx.x + k + 1;
-          mine = __reduce_max_sync(0xffffffffu, mine);
-          if ((threadIdx.x & 31) == 0) sh.warp_i[threadIdx.x >> 5] = mine;
-          __syncthreads();
-          listed = 0;
-          for (int w = 0; w < WARPS; ++w) listed = max(listed, sh.warp_i[w]);
-          if (threadIdx.x == 0) sh.told = sh.list[max(listed, 1) - 1];
-          __syncthreads();
-        }
-        if (!in_list) {
-          rd.sync();
-          cut = *rd.of(&sh.told, 0);
-        }
-      }
-    }
-    if (in_list) {
-      for (int i = threadIdx.x; i < listed; i += NT) {
-        const u64 c = sh.list[i];
-        take_better(best.v, best.i, sc.of(logit_of(c), index_of(c)), index_of(c));
-      }
-    } else {
-      draw(rd, sc, cut, best);
-    }
+    started();
   }
-
-  block_best(best.v, best.i, sh.warp_v, sh.warp_i);
-  if (in_list) {
-    if (threadIdx.x == 0) p.out[r] = best.i == 0x7fffffff ? 0 : best.i;
-    return;
+  if (cut != 0) {
+    best = hot ? draw_from<T>(sc, cut) : largest_of_row<T>();
+    block_best(best.v, best.i, sh.warp_v, sh.warp_i);
+    if (threadIdx.x == 0) { *of(&sh.part_v[sh.rank], 0) = best.v; *of(&sh.part_i[sh.rank], 0) = best.i; }
+    sync_row();
+    drawn = true;
+    if (sh.rank != 0) return;
   }
-  if (threadIdx.x == 0) { *rd.of(&sh.part_v[rd.rank], 0) = best.v; *rd.of(&sh.part_i[rd.rank], 0) = best.i; }
-  rd.sync();
-  if (rd.rank == 0 && threadIdx.x == 0) {
-    for (int b = 0; b < p.blocks; ++b) take_better(best.v, best.i, sh.part_v[b], sh.part_i[b]);
-    p.out[r] = best.i == 0x7fffffff ? 0 : best.i;
+  if (listed > 0) {
+    best = Best{-INFINITY, 0x7fffffff};
+    for (int i = threadIdx.x; i < listed; i += NT) {
+      const u64 c = sh.list[i];
+      take_better(best.v, best.i, sc.of(logit_of(c), sc.bits(index_of(c))), index_of(c));
+    }
+    block_best(best.v, best.i, sh.warp_v, sh.warp_i);
+  }
+  if (threadIdx.x == 0) {
+    if (drawn)
+      for (int b = 0; b < p.blocks; ++b) take_better(best.v, best.i, sh.part_v[b], sh.part_i[b]);
+    if (best.v > -INFINITY) p.out[r] = best.i;
   }
 }
 

@@ -10,11 +10,19 @@ __host__ __device__ __forceinline__ unsigned long long jv_mix64(unsigned long lo
   return z ^ (z >> 31);
 }
 
+// What the numbers of one (seed, counter) have in common, and the 64 random bits of its vocabulary index v: jv_uniform is
+// ((bits >> 40) + 0.5) / 2^24 in 32 bits.
+__host__ __device__ __forceinline__ unsigned long long jv_draw_base(unsigned long long seed, unsigned long long counter) {
+  return jv_mix64(seed + 0x9E3779B97F4A7C15ULL * (counter + 1));
+}
+__host__ __device__ __forceinline__ unsigned long long jv_draw_bits(unsigned long long base, unsigned long long v) {
+  return jv_mix64(base ^ (v * 0xD1342543DE82EF95ULL + 0x2545F4914F6CDD1DULL));
+}
+
 // Uniform in (0, 1) with 24 random bits.
 __host__ __device__ __forceinline__ float jv_uniform(unsigned long long seed, unsigned long long counter,
                                                      unsigned long long v) {
-  unsigned long long h = jv_mix64(seed + 0x9E3779B97F4A7C15ULL * (counter + 1));
-  h = jv_mix64(h ^ (v * 0xD1342543DE82EF95ULL + 0x2545F4914F6CDD1DULL));
+  const unsigned long long h = jv_draw_bits(jv_draw_base(seed, counter), v);
   return ((float)(unsigned)(h >> 40) + 0.5f) * (1.0f / 16777216.0f);
 }
 

@@ -30,105 +30,130 @@ __device__ __forceinline__ float logprob_of(float x, float largest, float log_su
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-template <typename T>
-__global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const ScoreParams p) {
-  extern __shared__ __align__(16) unsigned char memory[];
-  Shared& sh = *reinterpret_cast<Shared*>(memory);
-  pdl_trigger();
-  pdl_wait();
-  const int r = blockIdx.x / p.blocks;
-  Reader<T> rd;
-  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.stride;
-  rd.start(row, p.vocab, p.blocks, &sh);
-  // largest and sum of this thread's elements; what is no number (a NaN, infinity less infinity) adds nothing
+// Largest and sum of this thread's elements; what is no number (a NaN, infinity less infinity) adds nothing.
+template <typename T> __device__ __noinline__ float2 largest_and_sum() {
+  constexpr int VEC = 16 / (int)sizeof(T);
   float m = -INFINITY, s = 0.f;
-  rd.template each<8>([&](const auto& x, int) {
-    constexpr int V = sizeof(x) / sizeof(float);
+  each<T, 8>([&](const auto& x, int) {
     float big = x[0];
 #pragma unroll
-    for (int i = 1; i < V; ++i) big = fmaxf(big, x[i]);
+    for (int i = 1; i < VEC; ++i) big = fmaxf(big, x[i]);
     if (big > m) {
       s *= exp2_fast((m - big) * LOG2E);
       m = big;
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) s += exp2_fast(fmaxf(x[i] - m, -1000.f) * LOG2E);
+    for (int i = 0; i < VEC; ++i) s += exp2_fast(fmaxf(x[i] - m, -1000.f) * LOG2E);
   });
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float mb = warp_max(m);
-  double sum = m == mb ? (double)s : (double)(s * exp2_fast((m - mb) * LOG2E));
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) { sh.warp_v[warp] = mb; sh.warp_d[0][warp] = sum; }
-  rd.started();
-  rd.exchange_largest(m, p.top == 0 ? 1 : min((p.top - 1) / p.blocks + 1, MOST_OF_GROUPS), [&] {
-    if (threadIdx.x == 0) {
-      float block = -INFINITY;
-      for (int w = 0; w < WARPS; ++w) block = fmaxf(block, sh.warp_v[w]);
-      double all = 0.;
-      for (int w = 0; w < WARPS; ++w) all += sh.warp_v[w] == block ? sh.warp_d[0][w] : sh.warp_d[0][w] * (double)exp2_fast((sh.warp_v[w] - block) * LOG2E);
-      for (int b = 0; b < p.blocks; ++b) rd.of(&sh.part[rd.rank][0], b)[0] = all;
+  return make_float2(m, s);
+}
+
+template <typename T> __device__ __noinline__ float count_infinite() {
+  float count = 0.f;
+  each<T, 4>([&](const auto& x, int) {
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) count += x[i] == INFINITY ? 1.f : 0.f;
+  });
+  return count;
+}
+
+// Puts the tokens at or above `least`; a NaN is minus infinity, which may be among them.
+template <typename T> __device__ __noinline__ void list_first(float least) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int n = shared().n;
+  each<T, 4>([&](const auto& x, int at) {
+    float big = x[0];
+#pragma unroll
+    for (int i = 1; i < VEC; ++i) big = fmaxf(big, x[i]);
+    if (big >= least || least == -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float y = asked<false>(x[i], at + i, n);
+        if (y >= least) put(compose(y, at + i));
+      }
     }
   });
+}
+
+template <typename T>
+__global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const ScoreParams p) {
+  Shared& sh = shared();
+  constexpr int VEC = 16 / (int)sizeof(T);
+  pdl_trigger();
+  pdl_wait();
+  const int r = blockIdx.x / p.blocks;
+  const T* row = reinterpret_cast<const T*>(p.logits) + (size_t)r * p.stride;
+  begin(row, p.vocab, p.blocks);
+  const float2 mine = largest_and_sum<T>();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float of_warp = warp_max(mine.x);
+  double sum = mine.x == of_warp ? (double)mine.y : (double)(mine.y * exp2_fast((mine.x - of_warp) * LOG2E));
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) { sh.warp_v[warp] = of_warp; sh.warp_d[0][warp] = sum; }
+  started();
+  __syncthreads();
+  if (warp == 0) {
+    const float v = lane < WARPS ? sh.warp_v[lane] : -INFINITY, block = warp_max(v);
+    sum = lane < WARPS ? v == block ? sh.warp_d[0][lane] : sh.warp_d[0][lane] * (double)exp2_fast((v - block) * LOG2E) : 0.;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane < p.blocks) of(&sh.part[sh.rank][0], lane)[0] = sum;
+  }
+  exchange_largest(mine.x, p.top == 0 ? 1 : (p.top - 1) / p.blocks + 1);
+  if (p.top == 0 && sh.rank != 0 && sh.largest != INFINITY) return;
+  const float largest = sh.largest;
   sum = 0.;
-  for (int b = 0; b < p.blocks; ++b)
-    sum += sh.largest[b] == rd.largest ? sh.part[b][0] : sh.part[b][0] * (double)exp2_fast((sh.largest[b] - rd.largest) * LOG2E);
-  if (rd.largest == INFINITY) {                        // the infinite ones share the probability: how many they are
-    float count = 0.f;
-    rd.template each<4>([&](const auto& x, int) {
-      constexpr int V = sizeof(x) / sizeof(float);
-#pragma unroll
-      for (int i = 0; i < V; ++i) count += x[i] == INFINITY ? 1.f : 0.f;
-    });
-    double a = count, none = 0.;
-    rd.block_sums(a, none);
-    rd.sync();                                         // the others have read the last sums
+  for (int b = 0; b < p.blocks; ++b) {
+    const float v = sh.largest_of[b];
+    sum += v == largest ? sh.part[b][0] : sh.part[b][0] * (double)exp2_fast((v - largest) * LOG2E);
+  }
+  if (largest == INFINITY) {                           // the infinite ones share the probability: how many they are
+    const double2 a = block_sums((double)count_infinite<T>(), 0.);
+    sync_row();                                        // the others have read the last sums
     if (threadIdx.x == 0)
-      for (int b = 0; b < p.blocks; ++b) rd.of(&sh.part[rd.rank][0], b)[0] = a;
-    rd.sync();
+      for (int b = 0; b < p.blocks; ++b) of(&sh.part[sh.rank][0], b)[0] = a.x;
+    sync_row();
     sum = 0.;
     for (int b = 0; b < p.blocks; ++b) sum += sh.part[b][0];
   }
   const float log_sum = logf((float)sum);
-  if (rd.rank == 0 && threadIdx.x == 0) {
+  if (sh.rank == 0 && threadIdx.x == 0) {
     const int token = p.tokens[r];
     if (token < 0 || token >= p.vocab) {
       atomicOr(p.status, JV_STATUS_BAD_TOKEN);
       p.logprob[r] = NAN;
     } else {
-      p.logprob[r] = logprob_of(clean(to_f32(row[token])), rd.largest, log_sum);
+      p.logprob[r] = logprob_of(clean(to_f32(row[token])), largest, log_sum);
     }
   }
   if (p.top == 0) return;
 
-  const int j = (p.top - 1) / p.blocks + 1;
   bool found = false;
   unsigned total = 0;
-  if (j <= MOST_OF_GROUPS) {
-    const float least = rd.bound;
-    rd.template each<4>([&](const auto& x, int at) {
-      constexpr int V = sizeof(x) / sizeof(float);
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (clean(x[i]) >= least) rd.put(compose(clean(x[i]), at + i));
-    });
-    total = rd.send_list([] {});
+  if (countable((p.top - 1) / p.blocks + 1, p.blocks)) {
+    list_first<T>(sh.bound);
+    total = send_list();
     found = total <= (unsigned)LIST;
     if (!found && threadIdx.x == 0) sh.listed = 0;
   }
   if (!found) {
-    Range range;
-    const float wide = 6.f * (rd.largest - rd.bound);
-    rd.scale = 0.f;
-    rd.template narrow<false>((u64)KEY_LOWEST << INDEX_BITS, wide > 0.f ? (float)BINS / wide : 1.f, (unsigned)(LIST - p.top), range,
-                              [](unsigned, double) { return true; }, [&](unsigned n, double) { return n < (unsigned)p.top; });
-    total = rd.gather(range.lo, ~0ull);                // what lies above the range too: fewer than `top`
+    const float wide = 6.f * (largest - sh.bound);
+    if (threadIdx.x == 0) sh.scale = 0.f;
+    __syncthreads();
+    narrow<T, false>(LOWEST, wide > 0.f ? (float)BINS / wide : 1.f, (unsigned)(LIST - p.top), (double)p.top, -1., -1.);
+    // what lies above the range too: fewer than `top`
+    put_range<T, false, false>(LOWEST, [&](const auto& x, int at, unsigned which) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (which >> i & 1) put(compose(clean(x[i]), at + i));
+    });
+    total = send_list();
   }
-  if (rd.rank != 0) return;
-  rd.sort_list((int)total);
+  if (sh.rank != 0) return;
+  sort_list((int)total);
   for (int i = threadIdx.x; i < p.top; i += NT) {
     const u64 c = sh.list[i];
     p.top_tokens[(size_t)r * p.top + i] = index_of(c);
-    p.top_logprobs[(size_t)r * p.top + i] = logprob_of(logit_of(c), rd.largest, log_sum);
+    p.top_logprobs[(size_t)r * p.top + i] = logprob_of(logit_of(c), largest, log_sum);
   }
 }
 

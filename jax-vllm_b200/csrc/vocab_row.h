@@ -5,15 +5,18 @@
 // so that "the first tokens up to some boundary" are the tokens with c >= cut.  A NaN counts as minus infinity and -0 as 0.
 // A token weighs exp((x - largest) / T) in 32 bits; sums are 32-bit within a thread, 64-bit across threads, in a fixed order.
 //
-// Few first tokens are found in two passes.  In the first every block keeps the largest logit of each of its 128 groups of
-// threads.  The j-th largest of these has at least j tokens at or above it in that block, and about as many in a row whose
-// large logits lie anywhere; the lowest of the blocks' bounds therefore has at least j * blocks in the row.  The second
-// pass puts the tokens at or above the bound in a list, which the first block sorts.
+// Few first tokens are found in two passes.  In the first every thread keeps its largest logit.  The j-th largest of a block's
+// (of 128 groups of four threads, or of the threads where j is large) has at least j tokens at or above it in that block, and
+// not many more in a row whose large logits lie anywhere; the lowest of the blocks' bounds therefore has at least j * blocks
+// in the row.  The second pass puts the tokens at or above the bound in a list, which the first block sorts.
 //
 // Where that list does not do (the boundary lies deep in the row, or too many logits are equal), the boundary is found by
-// levels: every level cuts the range that holds it into 16 bins, sums up tokens and masses of each, and goes on in the bin
-// that holds the boundary, until that bin has few enough tokens to be sorted.  The bins are columns of shared memory that
+// levels: every level cuts the range that holds it into 31 bins, sums up the tokens or the masses of each, and goes on in the
+// bin that holds the boundary, until that bin has few enough tokens to be sorted.  The bins are columns of shared memory that
 // belong to one thread each: no atomics, no conflicts between banks, the same sums in every run.
+//
+// What all threads of a block know of its row stands in shared memory, and every pass over the row is a function of its own:
+// with all of it in one, the passes ran out of registers.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -28,10 +31,13 @@ constexpr int NT = 512, WARPS = NT / 32;               // threads of a block
 constexpr int MOST_BLOCKS = 8;                         // of a cluster
 constexpr int INDEX_BITS = 20, MAX_VOCAB = 1 << INDEX_BITS;
 constexpr unsigned KEY_LOWEST = 0x007fffffu;           // of minus infinity
-constexpr int BINS = 16, LIST = 1024;
+constexpr u64 LOWEST = (u64)KEY_LOWEST << INDEX_BITS;  // no token's number is smaller
+constexpr int BINS = 31, LIST = 2048;
 constexpr int GROUP = 4, GROUPS = NT / GROUP;          // lanes that share a largest logit; such groups of a block
-constexpr int MOST_OF_GROUPS = GROUPS * 7 / 8;         // the lowest of the groups' logits that is taken for a bound
+constexpr int FEW = GROUPS / 2;                        // tokens a block up to which the groups give the bound
+constexpr float HUGE_F = 3.402823466e38f;
 
+__device__ __forceinline__ float nan_f() { return __int_as_float(0x7fffffff); }
 __device__ __forceinline__ float clean(float x) { return x == x ? x + 0.f : -INFINITY; }
 __device__ __forceinline__ unsigned key_of(float x) {
   const unsigned u = __float_as_uint(x);
@@ -51,90 +57,65 @@ __device__ __forceinline__ float exp2_fast(float y) {  // two steps off at most;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e) : "f"(y));
   return e;
 }
-// exp((x - largest) / T) with scale = log2(e) / T; 1 for the largest itself (also where it is infinite).
-__device__ __forceinline__ float mass_of(float x, float largest, float scale) {
-  return x == largest ? 1.f : exp2_fast((x - largest) * scale);
-}
+// How far x lies below the largest logit; not at all where both are infinite (the difference is no number then).
+__device__ __forceinline__ float below(float x, float largest) { return fmaxf(largest - x, 0.f); }
 
-// The elements of a row that thread `me` of `all` reads, 16 bytes at a time from the first boundary on, AHEAD loads before
-// the first is used: f(values, index of the first), once for every load; elements before that boundary and behind the last
-// vector come one by one, last.  With WHOLE the lanes of a warp come together for every load: those with nothing left get
-// minus infinities behind the row's end.
-template <int AHEAD, bool WHOLE = false, typename T, typename F>
-__device__ __forceinline__ void for_row(const T* __restrict__ row, int n, int me, int all, F&& f) {
-  constexpr int VEC = 16 / (int)sizeof(T);
-  const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-  const int head = min(n, (VEC - off) % VEC);
-  const int vectors = (n - head) / VEC;
-  const uint4* body = reinterpret_cast<const uint4*>(row + head);
-  const int lane = WHOLE ? threadIdx.x & 31 : 0;
-  for (int j = me; j - lane < vectors; j += AHEAD * all) {
-    uint4 raw[AHEAD];
+// Sixteen bytes as 32-bit numbers.
+template <typename T> __device__ __forceinline__ void unpack(const uint4& raw, float (&x)[16 / sizeof(T)]) {
+  const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-      if (j + u * all < vectors) raw[u] = body[j + u * all];
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-      if (j - lane + u * all < vectors) {
-        float x[VEC];
-        if constexpr (sizeof(T) == 4) {
-          x[0] = __uint_as_float(raw[u].x); x[1] = __uint_as_float(raw[u].y);
-          x[2] = __uint_as_float(raw[u].z); x[3] = __uint_as_float(raw[u].w);
-        } else {
-          const unsigned w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-          }
-        }
-        const bool in = !WHOLE || j + u * all < vectors;
-        if (!in) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) x[i] = -INFINITY;
-        }
-        f(x, in ? head + (j + u * all) * VEC : MAX_VOCAB);
-      }
-  }
-  const int rest = n - vectors * VEC;                  // the head, and what follows the last vector
-  for (int e = me; e < rest; e += all) {
-    const int at = e < head ? e : e + vectors * VEC;
-    const float x[1] = {to_f32(row[at])};
-    f(x, at);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      x[i] = __uint_as_float(w[i]);
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
   }
 }
 
-struct Cell { float mass; unsigned count; };
-struct Sums { double mass; unsigned count, pad; };
+// A range of tokens that holds the boundary.  While the range is cut into bins of equal width it is given by the distance to
+// the row's largest logit, from <= largest - x < to (as 32 bits round it; no end where `to` is infinite), x no smaller than the
+// lowest logit asked for; once its logits crowd, by lo <= c <= hi.
+struct Range {
+  u64 lo, hi;
+  float from, to;
+  bool composed;
+  unsigned count;                                      // its tokens (where masses are summed: no fewer than that)
+  double above;                                        // tokens, or mass, above it
+};
 
 struct Shared {
   union {
-    Cell cells[BINS][NT];
+    float cells[BINS + 1][NT];                         // of a level: whole numbers or masses; the last row is not counted
     u64 own[LIST];                                     // this block's tokens on their way to the first block's list
   };
   u64 list[LIST];
-  Sums bins[2][MOST_BLOCKS][BINS];                     // what the blocks counted
+  double bins[2][MOST_BLOCKS][BINS];                   // what the blocks counted
   double part[MOST_BLOCKS][2];                         // sums that the blocks exchange
-  float largest[MOST_BLOCKS], bound[MOST_BLOCKS];
-  unsigned tokens[MOST_BLOCKS];
   float part_v[MOST_BLOCKS];
   int part_i[MOST_BLOCKS];
-  u64 told;                                            // the boundary, from the first block
-  double told_mass;
-  unsigned listed, mine, base;
-  float group[GROUPS];
+  unsigned tokens[MOST_BLOCKS];
+  float largest_of[MOST_BLOCKS], bound_of[MOST_BLOCKS];
+  alignas(16) float group[GROUPS];
   double warp_d[2][WARPS];
   float warp_v[32];
   int warp_i[32];
+  // the row: vectors of sixteen bytes that start on sixteen-byte boundaries, `off` elements of the first before the row; those
+  // from `whole` to `ragged` lie in it with all their elements
+  const void* row;
+  int n, off, vectors, whole, ragged, blocks, rank, parity;
+  float largest, scale, bound;                         // bound: at least `j * blocks` tokens are no smaller; scale: log2(e) / T
+  Range range;
+  u64 told;                                            // the boundary, from the first block
+  double all;                                          // tokens, or mass, of all that were asked for
+  unsigned listed, mine, base, best_key;
 };
+// The block's shared memory (named here, so that every function knows it for that).
+extern __shared__ __align__(16) unsigned char shared_bytes[];
+__device__ __forceinline__ Shared& shared() { return *reinterpret_cast<Shared*>(shared_bytes); }
 
-// The tokens lo <= c <= hi that hold the boundary, and what lies above them.
-struct Range {
-  u64 lo, hi;
-  double mass_above;
-  unsigned count_above, count;
-};
-
+// ---------------------------------------------------------------------------------------------------------- the cluster
 // jv_launch with clusters of `blocks` blocks along x (at most eight, and a divisor of the grid's x).
 template <typename... KArgs, typename... Args>
 static inline int launch_clusters(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, int blocks, cudaStream_t stream,
@@ -170,293 +151,581 @@ static inline int row_blocks(int rows, int vocab) {
   return blocks;
 }
 
-// The cluster that reads one row: `blocks` of NT threads.  Every member function is called by all threads of all blocks,
-// unless it says otherwise.
-template <typename T> struct Reader {
-  const T* row;
-  int n, rank, blocks, me, all, parity;
-  Shared* sh;
-  float largest, scale, bound;                         // bound: at least `j * blocks` tokens are no smaller
+// Every function below is called by all threads of all blocks of a row's cluster, unless it says otherwise.
 
-  __device__ __forceinline__ void sync() {
-    if (blocks > 1) cg::this_cluster().sync();
-    else __syncthreads();
+// Notes down the row, and tells the other blocks that this one runs.
+template <typename T> __device__ __forceinline__ void begin(const T* row, int n, int blocks) {
+  Shared& sh = shared();
+  if (threadIdx.x == 0) {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    sh.row = row;
+    sh.n = n;
+    sh.off = off;
+    sh.vectors = (off + n + VEC - 1) / VEC;
+    sh.whole = off == 0 ? 0 : 1;
+    sh.ragged = (off + n) / VEC;
+    sh.blocks = blocks;
+    sh.rank = blocks > 1 ? (int)cg::this_cluster().block_rank() : 0;
+    sh.parity = 0;
+    sh.listed = sh.mine = 0;
+    sh.best_key = KEY_LOWEST;
   }
-  template <typename V> __device__ __forceinline__ V* of(V* mine, int r) {
-    return blocks > 1 ? cg::this_cluster().map_shared_rank(mine, r) : mine;
-  }
-  // f(values, index of the first) for the elements of this thread
-  template <int AHEAD, typename F> __device__ __forceinline__ void each(F&& f) {
-    for_row<AHEAD>(row, n, me, all, f);
-  }
+  __syncthreads();
+  if (blocks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+}
+// Every block of the cluster runs, and has its counters at zero: their memory may be written.  Called once.
+__device__ __forceinline__ void started() {
+  if (shared().blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void sync_row() {
+  if (shared().blocks > 1) cg::this_cluster().sync();
+  else __syncthreads();
+}
+// The place of `mine` in the memory of block b.
+template <typename V> __device__ __forceinline__ V* of(V* mine, int b) {
+  return shared().blocks > 1 ? cg::this_cluster().map_shared_rank(mine, b) : mine;
+}
 
-  __device__ void start(const T* row_, int n_, int blocks_, Shared* sh_) {
-    row = row_; n = n_; blocks = blocks_; sh = sh_; parity = 0;
-    rank = blocks > 1 ? (int)cg::this_cluster().block_rank() : 0;
-    me = rank * NT + threadIdx.x;
-    all = blocks * NT;
-    if (threadIdx.x == 0) sh->listed = sh->mine = 0;
-    if (blocks > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
-  }
-  // Every block of the cluster runs, and has its counters at zero: their memory may be written.
-  __device__ __forceinline__ void started() {
-    if (blocks > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-    else __syncthreads();
-  }
-
-  // From the largest logit of every thread: the row's, and the bound that at least j tokens of every block reach (the lowest
-  // logit of all where a block has too few groups with any).  Holds one barrier of the cluster; before it, publish() may
-  // write to other blocks.
-  template <typename P> __device__ void exchange_largest(float m, int j, P&& publish) {
-    float g = m;
+// ---------------------------------------------------------------------------------------------------------- passes
+// Sixteen bytes of the row of which some lie outside it: those read as NaN.
+template <typename T> __device__ __noinline__ uint4 load_part(const T* row, int at, int n) {
+  unsigned w[4];
 #pragma unroll
-    for (int o = 1; o < GROUP; o *= 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if (threadIdx.x % GROUP == 0) sh->group[threadIdx.x / GROUP] = g;
-    __syncthreads();
-    // the place of group threadIdx.x / GROUP among all: each of its lanes compares with a share of the others
-    const int mine = threadIdx.x / GROUP;
-    int before = 0;
-#pragma unroll 8
-    for (int i = threadIdx.x % GROUP; i < GROUPS; i += GROUP) {
-      const float o = sh->group[i];
-      before += o > g || (o == g && i < mine);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      w[i] = at + i >= 0 && at + i < n ? reinterpret_cast<const unsigned*>(row)[at + i] : 0x7fffffffu;
+    } else {
+      const int l = at + 2 * i, h = l + 1;
+      w[i] = (l >= 0 && l < n ? reinterpret_cast<const unsigned short*>(row)[l] : 0x7fffu) |
+             (h >= 0 && h < n ? (unsigned)reinterpret_cast<const unsigned short*>(row)[h] : 0x7fffu) << 16;
     }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The vectors of the row that a thread reads one after the other: j, j + step, ...
+template <typename T> struct Vectors {
+  static constexpr int VEC = 16 / (int)sizeof(T);
+  const T* row;
+  int n, off, count, whole, ragged, step, start;
+
+  __device__ __forceinline__ Vectors() {
+    const Shared& sh = shared();
+    row = reinterpret_cast<const T*>(sh.row);
+    n = sh.n; off = sh.off; count = sh.vectors; whole = sh.whole; ragged = sh.ragged;
+    step = sh.blocks * NT;
+    start = sh.rank * NT + threadIdx.x;
+  }
+  __device__ __forceinline__ int first(int j) const { return j * VEC - off; }
+  // AHEAD of them from j on: all are asked for before the few that lie in the row in part.  NaNs where there is none.
+  template <int AHEAD> __device__ __forceinline__ void load(int j, uint4 (&raw)[AHEAD]) const {
 #pragma unroll
-    for (int o = 1; o < GROUP; o *= 2) before += __shfl_xor_sync(0xffffffffu, before, o);
-    if (threadIdx.x % GROUP == 0 && (before == 0 || before == j - 1)) {
-      for (int b = 0; b < blocks; ++b) {
-        if (before == 0) *of(&sh->largest[rank], b) = g;
-        if (before == j - 1) *of(&sh->bound[rank], b) = g;
+    for (int u = 0; u < AHEAD; ++u) {
+      const int k = j + u * step;
+      raw[u] = make_uint4(0x7fffffffu, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu);
+      if (k >= whole && k < ragged) raw[u] = *reinterpret_cast<const uint4*>(row + first(k));
+    }
+    if (j < whole || (j + (AHEAD - 1) * step >= ragged && ragged < count)) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int k = j + u * step;
+        if (k < count && !(k >= whole && k < ragged)) raw[u] = load_part(row, first(k), n);
       }
     }
-    publish();
-    sync();
-    largest = sh->largest[0];
-    bound = sh->bound[0];
-    for (int b = 1; b < blocks; ++b) {
-      largest = fmaxf(largest, sh->largest[b]);
-      bound = fminf(bound, sh->bound[b]);
-    }
-    largest += 0.f;                                    // never -0, as the keys
   }
+};
 
-  // Sums of a and b over the block, in a fixed order; valid in the first warp.
-  __device__ void block_sums(double& a, double& b) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// f(values, index of the first) for the vectors that this thread reads, AHEAD loads before the first is used; what lies outside
+// the row is NaN.  With WHOLE the lanes of a warp come together for every vector: those with none left get NaNs.
+template <typename T, int AHEAD, bool WHOLE = false, typename F> __device__ __forceinline__ void each(F&& f) {
+  const Vectors<T> v;
+  const int lane = WHOLE ? threadIdx.x & 31 : 0;
+  for (int j = v.start; j - lane < v.count; j += AHEAD * v.step) {
+    uint4 raw[AHEAD];
+    v.template load<AHEAD>(j, raw);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (j - lane + u * v.step < v.count) {
+        float x[Vectors<T>::VEC];
+        unpack<T>(raw[u], x);
+        f(x, v.first(j + u * v.step));
+      }
+  }
+}
+
+// A logit that may be counted.  Where masses are, minus infinity and NaN are never asked for; elsewhere a NaN of the row is
+// minus infinity, and one outside it stays what it is.
+template <bool MASS> __device__ __forceinline__ float asked(float x, int index, int n) {
+  return MASS || (unsigned)index >= (unsigned)n ? x : clean(x);
+}
+
+// This thread's largest logit.
+template <typename T> __device__ __noinline__ float my_largest() {
+  float m = -INFINITY;
+  each<T, 8>([&](const auto& x, int) {
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) m = fmaxf(m, x[i]);
+  });
+  return m;
+}
+
+// Whether a list of the tokens from the bound for j tokens a block up is likely to have room: of NT threads with their tokens
+// anywhere, NT * log(NT / (NT - j)) tokens are expected where j threads have one.
+__device__ __forceinline__ bool countable(int j, int blocks) {
+  return j < NT && (float)(blocks * NT) * -__logf(1.f - (float)j * (1.f / NT)) < 0.75f * LIST;
+}
+
+// From the largest logit of every thread: the row's, and the bound that at least j tokens of every block reach (minus infinity
+// where a block has too few threads with any).  Holds one barrier of the cluster.
+static __device__ __noinline__ void exchange_largest(float m, int j) {
+  Shared& sh = shared();
+  float g = m;
+#pragma unroll
+  for (int o = 1; o < GROUP; o *= 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+  const int part = threadIdx.x % GROUP, blocks = sh.blocks;
+  if (part == 0) sh.group[threadIdx.x / GROUP] = g;
+  __syncthreads();
+  // the groups above this one's largest, and those at it: each of its lanes compares with a share of the others
+  int both = 0;
+  const float4* others = reinterpret_cast<const float4*>(sh.group);
+#pragma unroll 4
+  for (int i = 0; i < GROUPS / 4 / GROUP; ++i) {
+    const float4 o = others[i * GROUP + part];
+    both += ((o.x > g) + (o.y > g) + (o.z > g) + (o.w > g)) << 16;
+    both += (o.x >= g) + (o.y >= g) + (o.z >= g) + (o.w >= g);
+  }
+#pragma unroll
+  for (int o = 1; o < GROUP; o *= 2) both += __shfl_xor_sync(0xffffffffu, both, o);
+  const int above = both >> 16, reach = both & 0xffff;
+  if (above == 0)                                      // (equal ones write the same)
+    for (int b = part; b < blocks; b += GROUP) *of(&sh.largest_of[sh.rank], b) = g;
+  if (j <= FEW) {
+    if (above < j && reach >= j)
+      for (int b = part; b < blocks; b += GROUP) *of(&sh.bound_of[sh.rank], b) = g;
+  } else {
+    // the threads' own largest: a key that j of them reach, by halves
+    unsigned lo = KEY_LOWEST, hi = 0xff800000u;        // at least j reach lo; fewer reach beyond hi
+    const unsigned mine = key_of(m + 0.f);
+    while (lo < hi) {
+      const unsigned mid = lo + (hi - lo) / 2 + 1;
+      const int c = __syncthreads_count(mine >= mid);
+      if (c >= j) lo = mid; else hi = mid - 1;
+      if (c >= j && c <= j + j / 16) break;
+    }
+    if (threadIdx.x < blocks) *of(&sh.bound_of[sh.rank], threadIdx.x) = value_of(lo);
+  }
+  sync_row();
+  if (threadIdx.x == 0) {
+    float l = sh.largest_of[0], low = sh.bound_of[0];
+    for (int b = 1; b < blocks; ++b) {
+      l = fmaxf(l, sh.largest_of[b]);
+      low = fminf(low, sh.bound_of[b]);
+    }
+    sh.largest = l + 0.f;                              // never -0, as the keys
+    sh.bound = low;
+  }
+  __syncthreads();
+}
+
+// Sums of a and b over the block, in a fixed order; valid in the first warp.
+static __device__ __noinline__ double2 block_sums(double a, double b) {
+  Shared& sh = shared();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int o = 16; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  __syncthreads();
+  if (lane == 0) { sh.warp_d[0][warp] = a; sh.warp_d[1][warp] = b; }
+  __syncthreads();
+  if (warp == 0) {
+    a = lane < WARPS ? sh.warp_d[0][lane] : 0.;
+    b = lane < WARPS ? sh.warp_d[1][lane] : 0.;
     for (int o = 16; o > 0; o >>= 1) {
       a += __shfl_xor_sync(0xffffffffu, a, o);
       b += __shfl_xor_sync(0xffffffffu, b, o);
     }
-    __syncthreads();
-    if (lane == 0) { sh->warp_d[0][warp] = a; sh->warp_d[1][warp] = b; }
-    __syncthreads();
-    if (warp == 0) {
-      a = lane < WARPS ? sh->warp_d[0][lane] : 0.;
-      b = lane < WARPS ? sh->warp_d[1][lane] : 0.;
-      for (int o = 16; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  return make_double2(a, b);
+}
+
+// ---------------------------------------------------------------------------------------------------------- the list
+// A token on its way to the list (any thread).
+__device__ __forceinline__ void put(u64 c) {
+  const unsigned at = atomicAdd(&shared().mine, 1u);
+  if (at < (unsigned)LIST) shared().own[at] = c;
+}
+
+// What every block has put goes to the first block's list, their number to `tokens` of every block.  Holds one barrier of the
+// cluster.  Returns the number of tokens put in the row: more than LIST, and the list is of no use.
+static __device__ __noinline__ unsigned send_list() {
+  Shared& sh = shared();
+  __syncthreads();
+  const unsigned count = sh.mine;
+  const int mine = min((int)count, LIST), blocks = sh.blocks;
+  if (threadIdx.x == 0) sh.base = count == 0 ? 0 : atomicAdd(of(&sh.listed, 0), count);
+  if (threadIdx.x < blocks) *of(&sh.tokens[sh.rank], threadIdx.x) = count;
+  __syncthreads();
+  const unsigned base = sh.base;
+  u64* list = of(&sh.list[0], 0);
+  for (int i = threadIdx.x; i < mine; i += NT)
+    if (base + i < (unsigned)LIST) list[base + i] = sh.own[i];
+  if (threadIdx.x == 0) sh.mine = 0;
+  sync_row();
+  unsigned total = 0;
+  for (int b = 0; b < blocks; ++b) total += sh.tokens[b];
+  return total;
+}
+
+// One pass instead of two, where one block reads a row: the bound for j tokens of what has been read so far, taken after the
+// first vectors and once more later, decides what is put, so that the list gets more tokens than it has to hold.  Minus
+// infinity is not put, nor what lies more than `deepest` below the largest.  Returns this thread's largest logit and, SUMMED,
+// the sum of its masses, relative to that one's.
+template <typename T, bool SUMMED> __device__ __noinline__ float2 put_once(int j, float deepest) {
+  constexpr int AHEAD = 4;
+  const Vectors<T> v;
+  const float scale = shared().scale;
+  float m = -INFINITY, s = 0.f, least = INFINITY;
+  const int rounds = (v.count + AHEAD * NT - 1) / (AHEAD * NT);
+  for (int k = 0; k < rounds; ++k) {
+    const int first = k * AHEAD * NT + threadIdx.x;
+    uint4 raw[AHEAD];
+    v.template load<AHEAD>(first, raw);
+    if (k == 0 || k == 3) {                            // what the first vectors hold above their own bound
+      float g = m;
+      if (k == 0) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          float x[v.VEC];
+          unpack<T>(raw[u], x);
+#pragma unroll
+          for (int i = 0; i < v.VEC; ++i) g = fmaxf(g, x[i]);
+        }
+      }
+      exchange_largest(g, j);
+      least = fmaxf(fmaxf(shared().bound, -HUGE_F), shared().largest - deepest);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      float x[v.VEC];
+      unpack<T>(raw[u], x);
+      float big = x[0];                                // (a NaN is passed over)
+#pragma unroll
+      for (int i = 1; i < v.VEC; ++i) big = fmaxf(big, x[i]);
+      if (SUMMED) {
+        if (big > m) s *= exp2_fast(-(fminf(big - m, HUGE_F) * scale));
+        const float to = fmaxf(big, m);
+#pragma unroll
+        for (int i = 0; i < v.VEC; ++i) s += x[i] > -INFINITY ? exp2_fast(-(below(x[i], to) * scale)) : 0.f;
+      }
+      m = fmaxf(m, big);
+      if (big >= least) {
+#pragma unroll
+        for (int i = 0; i < v.VEC; ++i)
+          if (x[i] >= least) put(compose(clean(x[i]), v.first(first + u * NT) + i));
       }
     }
   }
-
-  // A token on its way to the list (any thread).
-  __device__ __forceinline__ void put(u64 c) {
-    const unsigned at = atomicAdd(&sh->mine, 1u);
-    if (at < (unsigned)LIST) sh->own[at] = c;
-  }
-  // What every block has put goes to the first block's list, their number to `tokens` of every block.  Holds one barrier of
-  // the cluster.  Returns the number of tokens put in the row: more than LIST, and the list is of no use.
-  template <typename P> __device__ unsigned send_list(P&& publish) {
-    __syncthreads();
-    const unsigned count = sh->mine;
-    const int mine = min((int)count, LIST);
-    if (threadIdx.x == 0) sh->base = count == 0 ? 0 : atomicAdd(of(&sh->listed, 0), count);
-    if (threadIdx.x < blocks) *of(&sh->tokens[rank], threadIdx.x) = count;
-    publish();
-    __syncthreads();
-    const unsigned base = sh->base;
-    u64* list = of(&sh->list[0], 0);
-    for (int i = threadIdx.x; i < mine; i += NT)
-      if (base + i < (unsigned)LIST) list[base + i] = sh->own[i];
-    if (threadIdx.x == 0) sh->mine = 0;
-    sync();
-    unsigned total = 0;
-    for (int b = 0; b < blocks; ++b) total += sh->tokens[b];
-    return total;
-  }
-  // First block only: sorts its list, the largest first, and empties it for what is put next.
-  __device__ void sort_list(int m) {
-    int padded = 32;
-    while (padded < m) padded *= 2;
-    for (int i = m + threadIdx.x; i < padded; i += NT) sh->list[i] = 0;
-    if (threadIdx.x == 0) sh->listed = 0;
-    __syncthreads();
-    for (int size = 2; size <= padded; size *= 2)
-      for (int stride = size / 2; stride > 0; stride /= 2) {
-        for (int i = threadIdx.x; i < padded / 2; i += NT) {
-          const int a = 2 * i - (i & (stride - 1)), b = a + stride;
-          const bool down = (a & size) == 0;
-          const u64 u = sh->list[a], v = sh->list[b];
-          if ((u < v) == down) { sh->list[a] = v; sh->list[b] = u; }
-        }
-        __syncthreads();
-      }
-  }
-
-  // One level: tokens and masses of the 16 bins over the row, and the bin of the boundary: the lowest one that has tokens
-  // and for which before(tokens above, mass above) is true.  bin(x, index) in 0 .. 15 (15 the highest), or < 0: not counted.
-  // Takes the range over to that bin's sums and returns the bin; whole(tokens, mass) is told the sums of all bins first.
-  template <bool MASS, typename N, typename W, typename B>
-  __device__ int level(Range& r, N&& bin, W&& whole, B&& before) {
-    Cell* mine = &sh->cells[0][threadIdx.x];
-#pragma unroll
-    for (int b = 0; b < BINS; ++b) mine[b * NT] = Cell{0.f, 0u};
-    each<4>([&](const auto& x, int at) {
-      constexpr int V = sizeof(x) / sizeof(float);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float y = clean(x[i]);
-        const int b = bin(y, at + i);
-        if (b >= 0) {
-          Cell c = mine[b * NT];
-          ++c.count;
-          if (MASS) c.mass += mass_of(y, largest, scale);
-          mine[b * NT] = c;
-        }
-      }
-    });
-    __syncthreads();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int b = warp; b < BINS; b += WARPS) {
-      double q = 0;
-      unsigned c = 0;
-      for (int t = lane; t < NT; t += 32) {
-        const Cell v = sh->cells[b][t];
-        c += v.count;
-        q += (double)v.mass;
-      }
-      for (int o = 16; o > 0; o >>= 1) {
-        c += __shfl_xor_sync(0xffffffffu, c, o);
-        q += __shfl_xor_sync(0xffffffffu, q, o);
-      }
-      if (lane < blocks) *of(&sh->bins[parity][rank][b], lane) = Sums{q, c, 0u};
+  return make_float2(m, s);
+}
+// What has been put and is no smaller than `least` becomes the list (one block a row).  Returns the number of its tokens, or
+// LIST + 1 where more had been put than there was room for; both counters are at zero then.
+static __device__ __noinline__ unsigned keep_list(float least) {
+  Shared& sh = shared();
+  __syncthreads();
+  const unsigned count = sh.mine;
+  if (count <= (unsigned)LIST)
+    for (int i = threadIdx.x; i < (int)count; i += NT) {
+      const u64 c = sh.own[i];
+      if (logit_of(c) >= least) sh.list[atomicAdd(&sh.listed, 1u)] = c;
     }
-    sync();
-    // lane l has bin 15 - l: what lies above it is what the lanes before it have
-    double q = 0;
+  __syncthreads();
+  const unsigned kept = sh.listed;
+  __syncthreads();                                     // both counters are read: they may be set again
+  if (threadIdx.x == 0) sh.listed = sh.mine = 0;
+  return count <= (unsigned)LIST ? kept : LIST + 1;
+}
+
+// First block only: sorts its list of m tokens, the largest first, and empties it for what is put next.
+static __device__ __noinline__ void sort_list(int m) {
+  Shared& sh = shared();
+  if (threadIdx.x == 0) sh.listed = 0;
+  if (m <= NT / 4) {
+    // every token's place is the number of tokens before it: four lanes count them, a quarter each
+    const int i = threadIdx.x / 4;
+    const u64 c = i < m ? sh.list[i] : 0;
+    int place = 0;
+    for (int k = threadIdx.x % 4; k < m; k += 4) place += sh.list[k] > c;
+    place += __shfl_xor_sync(0xffffffffu, place, 1);
+    place += __shfl_xor_sync(0xffffffffu, place, 2);
+    __syncthreads();
+    if (i < m && threadIdx.x % 4 == 0) sh.list[place] = c;
+    __syncthreads();
+    return;
+  }
+  // bitonic: pairs less than a warp apart meet in registers
+  int padded = NT / 2;
+  while (padded < m) padded *= 2;
+  for (int i = m + threadIdx.x; i < padded; i += NT) sh.list[i] = 0;
+  __syncthreads();
+  for (int size = 32; size <= padded; size *= 2) {
+    for (int stride = size / 2; stride >= 32; stride /= 2) {
+      for (int i = threadIdx.x; i < padded / 2; i += NT) {
+        const int a = 2 * i - (i & (stride - 1)), b = a + stride;
+        const u64 u = sh.list[a], w = sh.list[b];
+        if ((u < w) == ((a & size) == 0)) { sh.list[a] = w; sh.list[b] = u; }
+      }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < padded; i += NT) {
+      u64 c = sh.list[i];
+      for (int part = size == 32 ? 2 : 32; part <= 32; part *= 2)
+        for (int stride = part / 2; stride > 0; stride /= 2) {
+          const u64 other = __shfl_xor_sync(0xffffffffu, c, stride);
+          const bool down = (i & (size == 32 ? part : size)) == 0, first = (i & stride) == 0;
+          if ((c < other) == (down == first)) c = other;
+        }
+      sh.list[i] = c;
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------- levels
+// The bin, 1 / per wide, of a distance d from `from` on; the last one takes what lies deeper.
+__device__ __forceinline__ int bin_of(float d, float from, float per) {
+  const float t = fminf((d - from) * per, (float)(BINS - 1));
+  return (int)(__float_as_uint(__fadd_rz(t, 8388608.f)) & 31u);
+}
+
+// Counts the tokens with c >= lo of the range [from, past) of distances in bins that are 1 / per wide; MASS: sums their masses.
+template <typename T, bool MASS> __device__ __noinline__ void count_linear(u64 lo, float from, float past, float per) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const float lowest = logit_of(lo), largest = shared().largest, scale = shared().scale;
+  const int n = shared().n;
+  const bool ragged = (lo & (MAX_VOCAB - 1)) != 0;     // the tokens asked for begin among equal logits
+  float* cells = &shared().cells[0][threadIdx.x];
+#pragma unroll
+  for (int b = 0; b < BINS; ++b) cells[b * NT] = 0.f;
+  each<T, 4>([&](const auto& x, int at) {
+    int bin[VEC];
+    float share[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float y = asked<MASS>(x[i], at + i, n), d = below(y, largest);
+      const bool in = y >= lowest && d >= from && !(d >= past);
+      const float t = in ? fminf((d - from) * per, (float)(BINS - 1)) : (float)BINS;
+      bin[i] = (int)(__float_as_uint(__fadd_rz(t, 8388608.f)) & 31u);
+      share[i] = exp2_fast(-(d * scale));
+    }
+    if (ragged) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (x[i] == lowest && compose(clean(x[i]), at + i) < lo) bin[i] = BINS;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      float& cell = cells[bin[i] * NT];
+      cell = MASS ? cell + share[i] : __uint_as_float(__float_as_uint(cell) + 1u);
+    }
+  });
+}
+// The same of the tokens lo <= c <= hi, in bins of 2^shift composed numbers.
+template <typename T, bool MASS> __device__ __noinline__ void count_composed(u64 lo, u64 hi, int shift) {
+  const float largest = shared().largest, scale = shared().scale, lowest = logit_of(lo);
+  const int n = shared().n;
+  float* cells = &shared().cells[0][threadIdx.x];
+#pragma unroll
+  for (int b = 0; b < BINS; ++b) cells[b * NT] = 0.f;
+  each<T, 2>([&](const auto& x, int at) {
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) {
+      const float y = asked<MASS>(x[i], at + i, n);
+      if (!(y >= lowest)) continue;
+      const u64 c = compose(clean(y), at + i);
+      if (c < lo || c > hi) continue;
+      float& cell = cells[(15 - (int)((c - lo) >> shift)) * NT];
+      cell = MASS ? cell + exp2_fast(-(below(y, largest) * scale)) : __uint_as_float(__float_as_uint(cell) + 1u);
+    }
+  });
+}
+
+// After every block has counted: the bin of the boundary, the last one that has tokens and before which `goal` (tokens, or
+// `part` of the whole mass where part >= 0) is not reached.  Takes range.above and range.count over to that bin's (the count
+// only where tokens are counted; else the bin's mass is returned in `inside`); `first`: `all` gets the sum of all bins.
+template <bool MASS> __device__ __noinline__ int choose(double goal, double part, bool first, double& inside) {
+  Shared& sh = shared();
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = sh.blocks, parity = sh.parity;
+  for (int b = warp; b < BINS; b += WARPS) {
+    float some[4] = {0.f, 0.f, 0.f, 0.f};
     unsigned c = 0;
-    if (lane < BINS)
-      for (int k = 0; k < blocks; ++k) {
-        const Sums s = sh->bins[parity][k][BINS - 1 - lane];
-        q += s.mass;
-        c += s.count;
-      }
-    parity ^= 1;
-    double q_to = q;
-    unsigned c_to = c;
-    for (int o = 1; o < BINS; o *= 2) {
-      const double qo = __shfl_up_sync(0xffffffffu, q_to, o);
-      const unsigned co = __shfl_up_sync(0xffffffffu, c_to, o);
-      if (lane >= o) { q_to += qo; c_to += co; }
+#pragma unroll
+    for (int t = 0; t < NT / 32; ++t) {
+      const float v = sh.cells[b][t * 32 + lane];
+      if (MASS) some[t % 4] += v;
+      else c += __float_as_uint(v);
     }
-    whole(__shfl_sync(0xffffffffu, c_to, BINS - 1), __shfl_sync(0xffffffffu, q_to, BINS - 1));
-    double q_above = __shfl_up_sync(0xffffffffu, q_to, 1);
-    unsigned c_above = __shfl_up_sync(0xffffffffu, c_to, 1);
-    q_above = r.mass_above + (lane == 0 ? 0. : q_above);
-    c_above = r.count_above + (lane == 0 ? 0u : c_above);
-    const unsigned holds = __ballot_sync(0xffffffffu, lane < BINS && c > 0 && before(c_above, q_above));
-    const int l = holds ? 31 - __clz(holds) : 0;
-    r.count_above = __shfl_sync(0xffffffffu, c_above, l);
-    r.mass_above = __shfl_sync(0xffffffffu, q_above, l);
-    r.count = __shfl_sync(0xffffffffu, c, l);
-    return BINS - 1 - l;
-  }
-
-  static __device__ __forceinline__ int linear_bin(float x, float top, float per) {
-    const float d = x >= top ? 0.f : (top - x) * per;
-    return BINS - 1 - min(BINS - 1, __float2int_rz(d));
-  }
-  // The smallest key from `a` to `z` whose value lies in linear bin b or above (that of z does).
-  static __device__ unsigned first_key(unsigned a, unsigned z, int b, float top, float per) {
-    const int lane = threadIdx.x & 31;
-    while (a < z) {
-      const unsigned step = (z - a + 31) / 32, p = min(z - 1, a + lane * step);
-      const unsigned yes = __ballot_sync(0xffffffffu, linear_bin(value_of(p), top, per) >= b);
-      if (yes == 0) { a = min(z - 1, a + 31 * step) + 1; continue; }
-      const int f = __ffs(yes) - 1;
-      const unsigned up = min(z - 1, a + f * step);
-      a = f == 0 ? a : min(z - 1, a + (f - 1) * step) + 1;
-      z = up;
+    double q;
+    if (MASS) {
+      q = (double)((some[0] + some[1]) + (some[2] + some[3]));
+      for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+    } else {
+      q = (double)__reduce_add_sync(0xffffffffu, c);
     }
-    return z;
+    if (lane < blocks) *of(&sh.bins[parity][sh.rank][b], lane) = q;
   }
-
-  // A level whose bins are 1 / per wide, from the range's highest logit down; the range becomes the boundary's bin.
-  template <bool MASS, typename W, typename B>
-  __device__ void linear_level(Range& r, float per, W&& whole, B&& before) {
-    const unsigned low = (unsigned)(r.lo >> INDEX_BITS), high = (unsigned)(r.hi >> INDEX_BITS);
-    const float top = value_of(high);
-    const u64 lo = r.lo, hi = r.hi;
-    const int b = level<MASS>(r, [&](float x, int i) {
-      const u64 c = compose(x, i);
-      return c >= lo && c <= hi ? linear_bin(x, top, per) : -1;
-    }, whole, before);
-    // (the last bin takes what lies deeper: it need not end at the range's lowest logit)
-    const u64 from = b == 0 ? 0 : (u64)first_key(low, high, b, top, per) << INDEX_BITS;
-    if (b < BINS - 1) r.hi = ((u64)first_key(low, high, b + 1, top, per) << INDEX_BITS) - 1;
-    r.lo = from > lo ? from : lo;
+  sync_row();
+  // what lies above a lane's bin is what the lanes before it have
+  double q = 0;
+  if (lane < BINS)
+    for (int k = 0; k < blocks; ++k) q += sh.bins[parity][k][lane];
+  double to = q;
+  for (int o = 1; o < 32; o *= 2) {
+    const double other = __shfl_up_sync(0xffffffffu, to, o);
+    if (lane >= o) to += other;
   }
+  const double all = first ? __shfl_sync(0xffffffffu, to, 31) : sh.all;
+  double above = __shfl_up_sync(0xffffffffu, to, 1);
+  above = sh.range.above + (lane == 0 ? 0. : above);
+  const double end = part >= 0. ? part * all : goal;
+  const unsigned holds = __ballot_sync(0xffffffffu, lane < BINS && q > 0. && (above == 0. || above < end));
+  const int l = holds ? 31 - __clz(holds) : 0;
+  above = __shfl_sync(0xffffffffu, above, l);
+  inside = __shfl_sync(0xffffffffu, q, l);
+  __syncthreads();                                     // the last level's sums are read
+  if (threadIdx.x == 0) {
+    sh.range.above = above;
+    sh.parity = parity ^ 1;
+    if (first) sh.all = all;
+  }
+  __syncthreads();
+  return l;
+}
 
-  // Finds a range of at most `most` tokens, among those with c >= lo, that holds the last token for which
-  // before(count, mass) of the tokens before it is true (it is true for the first token, and stays false once it is false).
-  // whole(count, mass) is told what all tokens with c >= lo make; where it says no, nothing is looked for.  The bins of
-  // the first level are 1 / per wide.
-  template <bool MASS, typename W, typename B>
-  __device__ bool narrow(u64 lo, float per, unsigned most, Range& r, W&& whole, B&& before) {
-    r = Range{lo, compose(largest, 0), 0., 0u, 0u};
-    bool wanted = true;
-    linear_level<MASS>(r, per, [&](unsigned c, double q) { wanted = whole(c, q); }, before);
-    if (!wanted) return false;
-    const auto nothing = [](unsigned, double) {};
-    for (int depth = 1; r.count > most; ++depth) {
-      const float high = logit_of(r.hi), wide = high - logit_of(r.lo);
-      const float finer = (float)BINS / wide;
-      if (depth < 3 && wide > 0.f && finer > 0.f && finer < INFINITY) {
-        linear_level<MASS>(r, finer, nothing, before);
-        continue;
+// The smallest distance in bin b or deeper, of those from `from` to `to` (which is given where there is none).
+static __device__ __noinline__ float first_distance(int b, float from, float to, float per) {
+  const int lane = threadIdx.x & 31;
+  unsigned a = __float_as_uint(from), z = __float_as_uint(to);
+  // it lies within a few steps of where it would without rounding
+  const float guess = from + (float)b / per;
+  if (guess > from && guess < to) {
+    const unsigned base = max(__float_as_uint(guess), 16u) - 16u, p = base + lane;
+    const unsigned yes = __ballot_sync(0xffffffffu, bin_of(__uint_as_float(min(max(p, a), z - 1)), from, per) >= b);
+    if (!(yes & 1u) && (yes >> 31)) { a = max(a, base); z = min(z, base + 31); }
+  }
+  while (a < z) {
+    const unsigned step = (z - a + 31) / 32, p = min(z - 1, a + lane * step);
+    const unsigned yes = __ballot_sync(0xffffffffu, bin_of(__uint_as_float(p), from, per) >= b);
+    if (yes == 0) { a = min(z - 1, a + 31 * step) + 1; continue; }
+    const int f = __ffs(yes) - 1;
+    if (f == 0) return __uint_as_float(a);
+    z = min(z - 1, a + f * step);
+    a = min(z, a + (f - 1) * step) + 1;
+  }
+  return __uint_as_float(z);
+}
+// The smallest key from `a` to `z` whose value lies nearer to the largest logit than `to` (that of z does, or none).
+static __device__ __noinline__ unsigned first_key(unsigned a, unsigned z, float to) {
+  const int lane = threadIdx.x & 31;
+  const float largest = shared().largest;
+  while (a < z) {
+    const unsigned step = (z - a + 31) / 32, p = min(z - 1, a + lane * step);
+    const unsigned yes = __ballot_sync(0xffffffffu, below(value_of(p), largest) < to);
+    if (yes == 0) { a = min(z - 1, a + 31 * step) + 1; continue; }
+    const int f = __ffs(yes) - 1;
+    if (f == 0) return a;
+    z = min(z - 1, a + f * step);
+    a = min(z, a + (f - 1) * step) + 1;
+  }
+  return z;
+}
+
+// Finds the range of at most `most` tokens, among those with c >= lo, that holds the last token before which the goal is not
+// reached: `goal` tokens, or (MASS) `goal` of the mass, or `part` of the mass of all tokens asked for where part >= 0.  `all` is
+// what all of them make; where that is no more than `plenty`, nothing is looked for.  The first level's bins are 1 / per wide.
+template <typename T, bool MASS> __device__ __noinline__ bool narrow(u64 lo, float per, unsigned most, double goal, double part, double plenty) {
+  Shared& sh = shared();
+  const float largest = sh.largest, deepest = below(logit_of(lo), largest);
+  Range r{lo, compose(largest, 0), 0.f, INFINITY, false, 0u, 0.};
+  if (threadIdx.x == 0) sh.range.above = 0.;
+  for (int depth = 0; depth == 0 || r.count > most; ++depth) {
+    if (depth > 0 && !r.composed) {
+      const float wide = fminf(r.to, deepest) - r.from;
+      per = (float)BINS / wide;
+      if (depth > 4 || !(wide > 0.f && per > 0.f && per < 1e37f && wide > 1e-6f * fminf(r.to, deepest))) {
+        // logits that crowd, or are equal: from here on by parts of the composed numbers, which end with a single one
+        const unsigned low = (unsigned)(lo >> INDEX_BITS), high = key_of(largest);
+        const u64 bottom = r.to == INFINITY ? lo : (u64)first_key(low, high, r.to) << INDEX_BITS;
+        if (r.from > 0.f) r.hi = ((u64)first_key(low, high, r.from) << INDEX_BITS) - 1;
+        r.lo = bottom > lo ? bottom : lo;
+        r.composed = true;
       }
-      // logits that crowd, or are equal: parts of the range of composed numbers, which ends with a single one
+    }
+    double inside = 0.;
+    float least;                                       // the deepest distance that the range may hold
+    if (!r.composed) {
+      const float from = r.from, to = r.to;
+      per = fminf(per, 1e37f);
+      count_linear<T, MASS>(lo, from, to == INFINITY ? nan_f() : to, per);
+      const int b = choose<MASS>(goal, part, depth == 0, inside);
+      if (depth == 0 && sh.all <= plenty) return false;
+      const float limit = fminf(to, HUGE_F);
+      if (b > 0) {
+        r.from = first_distance(b, from, limit, per);
+        if (r.from >= limit && bin_of(limit, from, per) < b) r.from = INFINITY;          // infinite distances alone
+      }
+      if (b < BINS - 1) {
+        r.to = first_distance(b + 1, from, limit, per);
+        if (r.to >= limit && bin_of(limit, from, per) <= b) r.to = to;
+      }
+      least = fminf(r.to, deepest);
+    } else {
       const u64 span = r.hi - r.lo, from = r.lo, to = r.hi;
       const int shift = max(0, 60 - __clzll((long long)span));
-      const int b = level<MASS>(r, [&](float x, int i) {
-        const u64 c = compose(x, i);
-        return c >= from && c <= to ? (int)((c - from) >> shift) : -1;
-      }, nothing, before);
-      r.lo = from + ((u64)b << shift);
+      count_composed<T, MASS>(from, to, shift);
+      const int b = choose<MASS>(goal, part, false, inside);
+      r.lo = from + ((u64)(15 - b) << shift);
       const u64 end = r.lo + ((1ull << shift) - 1);
       r.hi = end < to ? end : to;
+      least = below(logit_of(r.lo), largest);
     }
-    return true;
+    // no token of the range weighs less than one at its deepest
+    r.count = MASS ? (unsigned)fmin(inside * (double)exp2f(least * sh.scale) * 1.0001 + 1., 4e9) : (unsigned)inside;
   }
+  __syncthreads();
+  if (threadIdx.x == 0) { r.above = sh.range.above; sh.range = r; }
+  __syncthreads();
+  return true;
+}
 
-  // The tokens lo <= c <= hi go to the first block's list.
-  __device__ unsigned gather(u64 lo, u64 hi) {
-    const float low = logit_of(lo);
-    __syncthreads();                                   // the cells are read: their place is the list's too
-    each<4>([&](const auto& x, int at) {
-      constexpr int V = sizeof(x) / sizeof(float);
+// The tokens of the range, of those with c >= lo, are put; above(values, index of the first, which) is called for the vectors,
+// with a bit for each value that lies above the range, by whole warps where WHOLE.
+template <typename T, bool MASS, bool WHOLE, typename A> __device__ __forceinline__ void put_range(u64 lo, A&& above) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const Range& r = shared().range;
+  const bool composed = r.composed;
+  const float largest = shared().largest, lowest = logit_of(composed ? r.lo : lo), highest = composed ? logit_of(r.hi) : 0.f;
+  const float from = r.from, past = r.to == INFINITY ? nan_f() : r.to;
+  const u64 low = composed ? r.lo : lo, high = r.hi;
+  const int n = shared().n;
+  __syncthreads();                                     // the cells are read: their place is the list's too
+  each<T, WHOLE ? 2 : 4, WHOLE>([&](const auto& x, int at) {
+    unsigned which = 0;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float y = clean(x[i]);
-        if (y >= low) {
-          const u64 c = compose(y, at + i);
-          if (c >= lo && c <= hi) put(c);
-        }
+    for (int i = 0; i < VEC; ++i) {
+      const float y = asked<MASS>(x[i], at + i, n), d = below(y, largest);
+      bool over = y >= lowest && (composed ? y > highest : d < from);
+      if (y >= lowest && !over && (composed || !(d >= past))) {
+        const u64 c = compose(clean(y), at + i);
+        over = composed && c > high;
+        if (!over && c >= low) put(c);
       }
-    });
-    return send_list([] {});
-  }
-};
+      which |= over ? 1u << i : 0u;
+    }
+    above(x, at, which);
+  });
+}
 
 }  // namespace vocab
