@@ -23,6 +23,7 @@ struct Plane {
 };
 
 struct Pair { int src, dst, tokens; };                 // tokens < 0: the whole page
+struct Pairs { const int *src, *dst, *tokens; int n; };   // on the host; tokens may be null: whole pages
 
 template <int PLANES, int PAIRS> struct Job {
   Plane plane[PLANES];
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(THREADS) page_copy_kernel(const __grid_constan
 }
 
 template <typename V, int PLANES, int PAIRS>
-int copy_some(const Plane* planes, int n_planes, const Pair* pairs, int n_pairs, cudaStream_t stream) {
+int copy_some(const Plane* planes, int n_planes, const Pairs& pairs, int first, int n_pairs, cudaStream_t stream) {
   constexpr long long PIECE = 32 * UNROLL * (long long)sizeof(V);
   Job<PLANES, PAIRS> job;
   job.planes = n_planes;
@@ -78,7 +79,8 @@ int copy_some(const Plane* planes, int n_planes, const Pair* pairs, int n_pairs,
     total += (planes[p].page_bytes + PIECE - 1) / PIECE * planes[p].layers * n_pairs;
   }
   job.first[n_planes] = total;
-  for (int i = 0; i < n_pairs; ++i) job.pair[i] = pairs[i];
+  for (int i = 0; i < n_pairs; ++i)
+    job.pair[i] = Pair{pairs.src[first + i], pairs.dst[first + i], pairs.tokens != nullptr ? pairs.tokens[first + i] : -1};
   if (total == 0) return JV_OK;
   const long long wanted = (total + THREADS / 32 - 1) / (THREADS / 32), most = (long long)jv_multiprocessors() * 8;
   return jv_launch(page_copy_kernel<V, PLANES, PAIRS>, dim3((unsigned)(wanted < most ? wanted : most)), dim3(THREADS), 0, stream, job);
@@ -87,12 +89,12 @@ int copy_some(const Plane* planes, int n_planes, const Pair* pairs, int n_pairs,
 constexpr int FEW_PLANES = 4, FEW_PAIRS = 32, MANY_PLANES = 64, MANY_PAIRS = 1024;
 
 template <typename V>
-int copy_all(const Plane* planes, int n_planes, const Pair* pairs, int n_pairs, cudaStream_t stream) {
+int copy_all(const Plane* planes, int n_planes, const Pairs& pairs, cudaStream_t stream) {
   for (int p = 0; p < n_planes; p += MANY_PLANES)
-    for (int i = 0; i < n_pairs; i += MANY_PAIRS) {
-      const int np = n_planes - p < MANY_PLANES ? n_planes - p : MANY_PLANES, ni = n_pairs - i < MANY_PAIRS ? n_pairs - i : MANY_PAIRS;
-      const int rc = np <= FEW_PLANES && ni <= FEW_PAIRS ? copy_some<V, FEW_PLANES, FEW_PAIRS>(planes + p, np, pairs + i, ni, stream)
-                                                         : copy_some<V, MANY_PLANES, MANY_PAIRS>(planes + p, np, pairs + i, ni, stream);
+    for (int i = 0; i < pairs.n; i += MANY_PAIRS) {
+      const int np = n_planes - p < MANY_PLANES ? n_planes - p : MANY_PLANES, ni = pairs.n - i < MANY_PAIRS ? pairs.n - i : MANY_PAIRS;
+      const int rc = np <= FEW_PLANES && ni <= FEW_PAIRS ? copy_some<V, FEW_PLANES, FEW_PAIRS>(planes + p, np, pairs, i, ni, stream)
+                                                         : copy_some<V, MANY_PLANES, MANY_PAIRS>(planes + p, np, pairs, i, ni, stream);
       if (rc != JV_OK) return rc;
     }
   return JV_OK;
@@ -100,15 +102,12 @@ int copy_all(const Plane* planes, int n_planes, const Pair* pairs, int n_pairs, 
 
 }  // namespace
 
-// Launches that jv_page_copy makes for so many planes and pairs.
-JV_EXPORT int jv_page_copy_launches(int n_planes, int n_pairs) {
-  return ((n_planes + MANY_PLANES - 1) / MANY_PLANES) * ((n_pairs + MANY_PAIRS - 1) / MANY_PAIRS);
-}
-
 // planes: n_planes records of nine int64: from, to, from_layer, from_page, to_layer, to_page, page_bytes, token_bytes, layers.
-// pairs: n_pairs records of three int32: src, dst, tokens (< 0: the whole page).  Both on the host.
-JV_EXPORT int jv_page_copy(const long long* planes, int n_planes, const int* pairs, int n_pairs, cudaStream_t stream) {
+// src, dst, tokens: n_pairs int32 each (tokens null: whole pages).  All on the host.
+JV_EXPORT int jv_page_copy(const long long* planes, int n_planes, const int* src, const int* dst, const int* tokens, int n_pairs,
+                           cudaStream_t stream) {
   if (n_planes <= 0 || n_pairs <= 0) return JV_OK;
+  const Pairs pairs{src, dst, tokens, n_pairs};
   constexpr int SOME = 64;
   Plane buf[SOME];
   for (int base = 0; base < n_planes; base += SOME) {
@@ -119,11 +118,10 @@ JV_EXPORT int jv_page_copy(const long long* planes, int n_planes, const int* pai
       buf[p] = Plane{reinterpret_cast<const char*>(r[0]), reinterpret_cast<char*>(r[1]), r[2], r[3], r[4], r[5], r[6], r[7], (int)r[8]};
       for (int k = 0; k < 8; ++k) all |= (unsigned long long)r[k];
     }
-    const Pair* pr = reinterpret_cast<const Pair*>(pairs);
-    const int rc = all % 16 == 0  ? copy_all<uint4>(buf, n, pr, n_pairs, stream)
-                   : all % 4 == 0 ? copy_all<uint32_t>(buf, n, pr, n_pairs, stream)
-                   : all % 2 == 0 ? copy_all<uint16_t>(buf, n, pr, n_pairs, stream)
-                                  : copy_all<uint8_t>(buf, n, pr, n_pairs, stream);
+    const int rc = all % 16 == 0  ? copy_all<uint4>(buf, n, pairs, stream)
+                   : all % 4 == 0 ? copy_all<uint32_t>(buf, n, pairs, stream)
+                   : all % 2 == 0 ? copy_all<uint16_t>(buf, n, pairs, stream)
+                                  : copy_all<uint8_t>(buf, n, pairs, stream);
     if (rc != JV_OK) return rc;
   }
   return JV_OK;

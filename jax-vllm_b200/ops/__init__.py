@@ -12,13 +12,14 @@ kernel of this package.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import math
-import operator
 import os
 import struct
 from ctypes import c_char_p, c_float, c_int, c_longlong, c_void_p
 
+import numpy as np
 import torch
 
 from ..csrc import build as _build
@@ -2539,32 +2540,38 @@ MOST_TOP = 128                     # likeliest tokens a row that `token_logprobs
 
 
 def _logit_rows(who: str, logits: torch.Tensor, values) -> tuple:
-    """(rows, vocab, elements between rows) of a matrix of logits whose rows are contiguous; `values`: (name, tensor, dtype)
-    of what stands beside them, one number a row."""
+    """(rows, vocab, elements between rows, type code) of a matrix of logits whose rows are contiguous; `values`: (name,
+    tensor, dtype) of what stands beside them, one number a row."""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
         raise KernelError(f"{who}: logits are a matrix [rows, vocab]")
     rows, vocab = logits.shape
     if vocab < 1 or vocab > MOST_VOCAB:
         raise KernelError(f"{who}: rows of 1 to {MOST_VOCAB} logits, got {vocab}")
-    if logits.dtype not in DTYPE_CODE:
+    code = DTYPE_CODE.get(logits.dtype)
+    if code is None:
         raise KernelError(f"{who}: logits must be float32 or bfloat16, got {logits.dtype}")
-    stride = logits.stride(0) if rows > 1 else vocab
-    if (vocab > 1 and logits.stride(1) != 1) or stride < vocab:
-        raise KernelError(f"{who}: the logits of a row must be contiguous, and rows must not overlap")
+    stride = vocab
+    if not logits.is_contiguous():
+        stride = logits.stride(0) if rows > 1 else vocab
+        if (vocab > 1 and logits.stride(1) != 1) or stride < vocab:
+            raise KernelError(f"{who}: the logits of a row must be contiguous, and rows must not overlap")
+    device = logits.get_device()
     for name, t, dtype in values:
-        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous():
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.dim() != 1 or t.numel() != rows or not t.is_contiguous():
             raise KernelError(f"{who}: {name} must be {dtype}, contiguous, one value for each of the {rows} rows")
-        if t.device != logits.device:
+        if t.get_device() != device:
             raise KernelError(f"{who}: {name} is on {t.device}, the logits on {logits.device}")
-    _on_current_device(who, logits)
-    return rows, vocab, stride
+    _on_current_device(who, device)
+    return rows, vocab, stride, code
 
 
-def _on_current_device(who: str, t: torch.Tensor) -> None:
-    if not t.is_cuda:
+def _on_current_device(who: str, index: int) -> None:
+    """`index`: what a tensor's `get_device` gives.  A launch goes to the current device's stream."""
+    if index < 0:
         raise KernelError(f"{who}: the tensors must be CUDA tensors (this engine has no CPU path)")
-    if t.device.index != torch.cuda.current_device():
-        raise KernelError(f"{who}: the tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    current = _raw_device() if _raw_device is not None else torch.cuda.current_device()
+    if index != current:
+        raise KernelError(f"{who}: the tensors are on cuda:{index}, the current device is cuda:{current}")
 
 
 def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torch.Tensor, top_p: torch.Tensor, min_p: torch.Tensor,
@@ -2580,14 +2587,14 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
     The draw is the kept token with the largest logit / temperature - log(-log(u)), where u depends on (seed, counter,
     token id) only: the numbers of `sample`, whose tokens a row without filters gets.  A temperature of 0 takes the largest
     logit.  A NaN counts as minus infinity; a row with nothing else gives token 0."""
-    rows, vocab, stride = _logit_rows("sample_filtered", logits, (
+    rows, vocab, stride, code = _logit_rows("sample_filtered", logits, (
         ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
         ("min_p", min_p, torch.float32), ("seeds", seeds, torch.int64), ("counters", counters, torch.int64)))
     out = torch.empty(rows, dtype=torch.int32, device=logits.device)
     if rows == 0:
         return out
     f = _fn("sample_filtered", "jv_sample_filtered", _SAMPLE_FILTERED_TYPES)
-    _check(f(logits.data_ptr(), DTYPE_CODE[logits.dtype], stride, rows, vocab, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
+    _check(f(logits.data_ptr(), code, stride, rows, vocab, temperature.data_ptr(), top_k.data_ptr(), top_p.data_ptr(),
              min_p.data_ptr(), seeds.data_ptr(), counters.data_ptr(), out.data_ptr(), 0, _stream()), "sample_filtered")
     return out
 
@@ -2597,7 +2604,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     float32 or bfloat16 logits, and the `top` likeliest tokens (at most 128) with theirs, equal ones in the order of their
     indices.  32-bit.  A NaN counts as minus infinity; in a row with nothing else every logprob is minus infinity.  A token
     outside the vocabulary sets the status word and gives NaN."""
-    rows, vocab, stride = _logit_rows("token_logprobs", logits, (("tokens", tokens, torch.int32),))
+    rows, vocab, stride, code = _logit_rows("token_logprobs", logits, (("tokens", tokens, torch.int32),))
     top = int(top)
     if top < 0 or top > MOST_TOP or top > vocab:
         raise KernelError(f"token_logprobs: top must be 0 to {min(MOST_TOP, vocab)}, got {top}")
@@ -2608,45 +2615,43 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if rows == 0:
         return logprob, top_tokens, top_logprobs
     f = _fn("token_logprobs", "jv_token_logprobs", _TOKEN_LOGPROBS_TYPES)
-    _check(f(logits.data_ptr(), DTYPE_CODE[logits.dtype], stride, rows, vocab, tokens.data_ptr(), top, logprob.data_ptr(),
+    _check(f(logits.data_ptr(), code, stride, rows, vocab, tokens.data_ptr(), top, logprob.data_ptr(),
              top_tokens.data_ptr(), top_logprobs.data_ptr(), _status_ptr(device), 0, _stream()), "token_logprobs")
     return logprob, top_tokens, top_logprobs
 
 
 # ------------------------------------------------------------------- copies inside a cache
-def _index_list(who: str, name: str, ids) -> list:
-    """`ids` as a list of ints: indices that the host knows (a launch carries them as parameters)."""
-    if isinstance(ids, torch.Tensor):
-        if ids.is_cuda or ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64):
-            raise KernelError(f"{who}: {name} must be integers on the host")
-        return ids.tolist()
-    ids = list(ids)
-    if not all(type(i) is int for i in ids):
-        try:
-            ids = [operator.index(i) for i in ids]
-        except TypeError:
-            raise KernelError(f"{who}: {name} must be integers") from None
-    return ids
-
-
 def check_copies(who: str, src, dst, n_src: int, n_dst: int, apart: bool, tokens=None, most: int = 0) -> tuple:
-    """(src, dst, tokens) as lists, after the checks of a copy: indices that exist, no destination twice and, unless sources
+    """(sources, destinations, numbers of tokens or None) of a copy as arrays of 32-bit integers, after the checks: integers
+    that the host knows (a launch carries them as parameters), indices that exist, no destination twice and, unless sources
     and destinations are `apart`, none that is a source too."""
-    src, dst = _index_list(who, "src", src), _index_list(who, "dst", dst)
-    if len(src) != len(dst):
-        raise KernelError(f"{who}: {len(src)} sources and {len(dst)} destinations")
-    if tokens is not None:
-        tokens = _index_list(who, "tokens", tokens)
-        if len(tokens) != len(src):
-            raise KernelError(f"{who}: one number of tokens per pair")
-        if tokens and (min(tokens) < 0 or max(tokens) > most):
-            raise KernelError(f"{who}: a page holds 0 to {most} tokens")
-    if not src:
+    arrays = []
+    for name, ids in (("src", src), ("dst", dst), ("tokens", tokens)):
+        if ids is None:
+            arrays.append(None)
+            continue
+        if isinstance(ids, torch.Tensor):
+            if ids.is_cuda or ids.dim() != 1 or ids.dtype not in (torch.int32, torch.int64):
+                raise KernelError(f"{who}: {name} must be integers on the host")
+            ids = ids.tolist()
+        try:
+            arrays.append(array.array("i", ids))
+        except (TypeError, OverflowError):
+            raise KernelError(f"{who}: {name} must be 32-bit integers") from None
+    src, dst, tokens = arrays
+    n = len(src)
+    if len(dst) != n or (tokens is not None and len(tokens) != n):
+        raise KernelError(f"{who}: as many destinations (and numbers of tokens) as sources")
+    if n == 0:
         return src, dst, tokens
-    if min(src) < 0 or max(src) >= n_src or min(dst) < 0 or max(dst) >= n_dst:
+    # (numpy's reductions take longer to begin and less for each number)
+    low, high = (min, max) if n < 64 else (lambda a: np.frombuffer(a, np.int32).min(), lambda a: np.frombuffer(a, np.int32).max())
+    if tokens is not None and (low(tokens) < 0 or high(tokens) > most):
+        raise KernelError(f"{who}: a page holds 0 to {most} tokens")
+    if low(src) < 0 or high(src) >= n_src or low(dst) < 0 or high(dst) >= n_dst:
         raise KernelError(f"{who}: sources lie in [0, {n_src}), destinations in [0, {n_dst})")
     written = set(dst)
-    if len(written) != len(dst):
+    if len(written) != n:
         raise KernelError(f"{who}: a destination is given twice")
     if not apart and not written.isdisjoint(src):
         raise KernelError(f"{who}: a destination is a source too")
@@ -2659,15 +2664,34 @@ def _span(t: torch.Tensor) -> tuple:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
-def _copy_planes(who: str, planes: list, src: list, dst: list, tokens) -> None:
-    """planes: nine numbers each, as csrc/page_copy.cu takes them."""
-    n = len(src)
-    pairs = [0] * (3 * n)
-    pairs[0::3], pairs[1::3], pairs[2::3] = src, dst, tokens if tokens is not None else [-1] * n
-    flat = [v for plane in planes for v in plane]
-    launches = -(-len(planes) // 64) * -(-n // 1024)
-    f = _fn("page_copy", "jv_page_copy", [c_char_p, c_int, c_char_p, c_int, c_void_p])
-    _check(f(struct.pack(f"{len(flat)}q", *flat), len(planes), struct.pack(f"{3 * n}i", *pairs), n, _stream()), who, launches=launches)
+_PAGE_COPY_TYPES = [c_char_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p]
+
+
+def _copy_planes(who: str, planes: list, pairs: tuple) -> None:
+    """planes: nine numbers for each, one after the other, as csrc/page_copy.cu takes them."""
+    src, dst, tokens = pairs
+    n_planes, n_pairs = len(planes) // 9, len(src)
+    f = _fn("page_copy", "jv_page_copy", _PAGE_COPY_TYPES)
+    _check(f(struct.pack(f"{len(planes)}q", *planes), n_planes, src.buffer_info()[0], dst.buffer_info()[0],
+             0 if tokens is None else tokens.buffer_info()[0], n_pairs, _stream()), who, launches=-(-n_planes // 64) * -(-n_pairs // 1024))
+
+
+def _page_strides(who: str, t: torch.Tensor) -> tuple:
+    """(elements from one layer to the next, from one page to the next, of a page) of a store whose pages are contiguous and
+    do not overlap."""
+    shape = t.shape
+    layers, pages, page = shape[0], shape[1], math.prod(shape[2:])
+    if t.is_contiguous():
+        return pages * page, page, page
+    s0, s1, inner, size = t.stride(0), t.stride(1), t.stride()[2:], 1
+    for n, s in zip(reversed(shape[2:]), reversed(inner)):
+        if n != 1 and s != size:
+            raise KernelError(f"{who}: a page must be contiguous")
+        size *= n
+    if (layers > 1 and s0 < page) or (pages > 1 and s1 < page) or \
+            (layers > 1 and pages > 1 and s0 < (pages - 1) * s1 + page and s1 < (layers - 1) * s0 + page):
+        raise KernelError(f"{who}: pages must not overlap")
+    return s0, s1, page
 
 
 def copy_pages(stores, src, dst, tokens=None, into=None) -> None:
@@ -2680,34 +2704,34 @@ def copy_pages(stores, src, dst, tokens=None, into=None) -> None:
     to = stores if into is None else list(into)
     if not stores or len(to) != len(stores):
         raise KernelError("copy_pages: a list of stores, and as many to copy into")
-    for a, b in zip(stores, to):
-        if not isinstance(a, torch.Tensor) or not isinstance(b, torch.Tensor) or a.dim() < 3 or a.shape[:1] + a.shape[2:] != b.shape[:1] + b.shape[2:] \
-                or a.dtype != b.dtype or a.device != b.device:
-            raise KernelError("copy_pages: stores are [layers, pages, page_size, ...]; what is copied into has the same type, device and shape but for the pages")
-        if a.shape[1:3] != stores[0].shape[1:3] or b.shape[1] != to[0].shape[1]:
+    planes, n_src, n_dst, page_size = [], 0, 0, 0
+    for k, a in enumerate(stores):
+        if not isinstance(a, torch.Tensor) or a.dim() < 3:
+            raise KernelError("copy_pages: stores are [layers, pages, page_size, ...]")
+        b, shape = to[k], a.shape
+        if b is not a and (not isinstance(b, torch.Tensor) or b.dim() != a.dim() or shape[:1] + shape[2:] != b.shape[:1] + b.shape[2:]
+                           or a.dtype is not b.dtype or a.device != b.device):
+            raise KernelError("copy_pages: what is copied into has the same type, device and shape as the store, but for the pages")
+        if k == 0:
+            n_src, n_dst, page_size = shape[1], b.shape[1], shape[2]
+        elif shape[1] != n_src or b.shape[1] != n_dst or shape[2] != page_size:
             raise KernelError("copy_pages: all stores have the same number of pages and of tokens in a page")
-    src, dst, tokens = check_copies("copy_pages", src, dst, stores[0].shape[1], to[0].shape[1], into is not None, tokens, stores[0].shape[2])
-    planes = []
-    for a, b in zip(stores, to):
-        _on_current_device("copy_pages", a)
-        page = math.prod(a.shape[2:])
-        for t in (a, b):
-            if t.numel() and not t[0, 0].is_contiguous():
-                raise KernelError("copy_pages: a page must be contiguous")
-            (n0, n1), (s0, s1) = t.shape[:2], t.stride()[:2]
-            if t.numel() and not (n0 == 1 or s0 >= (n1 - 1) * s1 + page) and not (n1 == 1 or s1 >= (n0 - 1) * s0 + page) \
-                    or (n0 > 1 and s0 < page) or (n1 > 1 and s1 < page):
-                raise KernelError("copy_pages: pages must not overlap")
         size = a.element_size()
-        planes.append((a.data_ptr(), b.data_ptr(), a.stride(0) * size, a.stride(1) * size, b.stride(0) * size, b.stride(1) * size,
-                       page * size, page // max(1, a.shape[2]) * size, a.shape[0]))
+        layer, page, row = _page_strides("copy_pages", a)
+        to_layer, to_page, _ = (layer, page, row) if b is a else _page_strides("copy_pages", b)
+        if row and shape[0]:
+            planes += (a.data_ptr(), b.data_ptr(), layer * size, page * size, to_layer * size, to_page * size, row * size, row // page_size * size,
+                       shape[0])
+    pairs = check_copies("copy_pages", src, dst, n_src, n_dst, into is not None, tokens, page_size)
+    for a in stores:
+        _on_current_device("copy_pages", a.get_device())
     if into is not None:
         spans = [_span(t) for t in to if t.numel()]
         for x in (_span(t) for t in stores if t.numel()):
             if any(x[0] < y[1] and y[0] < x[1] for y in spans):
                 raise KernelError("copy_pages: the stores to copy into must lie apart from the others in memory")
-    if src and all(p[6] and p[8] for p in planes):
-        _copy_planes("copy_pages", planes, src, dst, tokens)
+    if pairs[0] and planes:
+        _copy_planes("copy_pages", planes, pairs)
 
 
 def copy_slots(states, src, dst) -> None:
@@ -2717,19 +2741,25 @@ def copy_slots(states, src, dst) -> None:
     if not states:
         raise KernelError("copy_slots: a list of state tensors")
     slots = states[0].shape[0] if isinstance(states[0], torch.Tensor) and states[0].dim() else 0
-    src, dst, _ = check_copies("copy_slots", src, dst, slots, slots, False)
-    planes = []
+    pairs = check_copies("copy_slots", src, dst, slots, slots, False)
+    planes, device = [], None
     for t in states:
         if not isinstance(t, torch.Tensor) or t.dim() < 1 or t.shape[0] != slots:
             raise KernelError("copy_slots: all states are [slots, ...] with the same number of slots")
-        _on_current_device("copy_slots", t)
-        row = math.prod(t.shape[1:])
-        if t.numel() and not t[0].is_contiguous():
-            raise KernelError("copy_slots: a row must be contiguous")
-        if slots > 1 and t.stride(0) < row:
-            raise KernelError("copy_slots: rows must not overlap")
-        size = t.element_size()
-        if row:
-            planes.append((t.data_ptr(), t.data_ptr(), 0, t.stride(0) * size, 0, t.stride(0) * size, row * size, row * size, 1))
-    if src and planes:
-        _copy_planes("copy_slots", planes, src, dst, None)
+        if device is None or t.get_device() != device:
+            device = t.get_device()
+            _on_current_device("copy_slots", device)
+        at, size = t.data_ptr(), t.nbytes
+        if not size:
+            continue
+        row = size // slots
+        step = row
+        if not t.is_contiguous():
+            step = t.stride(0) * t.element_size()
+            if not t[0].is_contiguous():
+                raise KernelError("copy_slots: a row must be contiguous")
+            if slots > 1 and step < row:
+                raise KernelError("copy_slots: rows must not overlap")
+        planes += (at, at, 0, step, 0, step, row, row, 1)
+    if pairs[0] and planes:
+        _copy_planes("copy_slots", planes, pairs)

@@ -10,7 +10,7 @@ from jax_vllm_b200 import ops
 @pytest.mark.parametrize("src,dst,apart,tokens", [
     ([0, 1], [2], False, None), ([0], [10], False, None), ([10], [0], False, None), ([-1], [0], False, None), ([0], [-1], False, None),
     ([0, 1], [5, 5], False, None), ([0, 1], [5, 5], True, None), ([0, 1], [1, 2], False, None), ([3], [3], False, None), ([0.5], [1], False, None),
-    (["a"], [1], False, None), ([0], [1], False, [17]), ([0], [1], False, [-1]), ([0], [1], False, [1, 2]), (torch.tensor([0.0]), [1], False, None),
+    (["a"], [1], False, None), ([1 << 40], [1], False, None), ([None], [1], False, None), ([0], [1], False, [17]), ([0], [1], False, [-1]), ([0], [1], False, [1, 2]), (torch.tensor([0.0]), [1], False, None),
     (torch.tensor([[0]]), [1], False, None)])
 def test_copies_that_are_refused(src, dst, apart, tokens):
     with pytest.raises(ops.KernelError):
@@ -18,11 +18,22 @@ def test_copies_that_are_refused(src, dst, apart, tokens):
 
 
 def test_indices_of_any_integer_kind():
-    for src in ([1, 1], (1, 1), torch.tensor([1, 1]), torch.tensor([1, 1], dtype=torch.int32), np.array([1, 1]), range(1, 3)):
+    for src in ([1, 1], (1, 1), torch.tensor([1, 1]), torch.tensor([1, 1], dtype=torch.int32), np.array([1, 1]), iter([1, 1])):
         got = ops.check_copies("copy", src, [5, 6], 10, 10, False, [16, 0], 16)
-        assert got[1:] == ([5, 6], [16, 0]) and len(got[0]) == 2 and all(type(i) is int for i in got[0])
-    assert ops.check_copies("copy", [3, 1], [1, 3], 10, 10, True) == ([3, 1], [1, 3], None)
-    assert ops.check_copies("copy", [], [], 0, 0, False) == ([], [], None)
+        assert [list(a) for a in got] == [[1, 1], [5, 6], [16, 0]]
+    many = list(range(100))
+    got = ops.check_copies("copy", many, [i + 100 for i in many], 100, 200, True)
+    assert list(got[0]) == many and list(got[1]) == list(range(100, 200)) and got[2] is None
+    assert [len(a) for a in ops.check_copies("copy", [], [], 0, 0, False)[:2]] == [0, 0]
+
+
+@pytest.mark.parametrize("change", [dict(src=100), dict(src=-1), dict(dst=200), dict(dst=-1), dict(dst=150), dict(tokens=17), dict(tokens=-1)])
+def test_one_bad_number_among_many_is_refused(change):
+    lists = dict(src=list(range(100)), dst=list(range(100, 200)), tokens=[3] * 100)
+    for name, value in change.items():
+        lists[name][41] = value
+    with pytest.raises(ops.KernelError):
+        ops.check_copies("copy", lists["src"], lists["dst"], 100, 200, True, lists["tokens"], 16)
 
 
 def test_tensors_on_the_host_are_refused():
