@@ -42,6 +42,11 @@ def main(argv=None) -> int:
     p.add_argument("--prompt-ids", action="append", default=[], help="a prompt as token ids, e.g. 1,2,3 (repeatable)")
     p.add_argument("--prompt", action="append", default=[], help="a prompt as text (needs the folder's tokenizer)")
     p.add_argument("--temperature", type=float, default=0.0)
+    p.add_argument("--top-k", type=int, default=0, help="draw from the k likeliest tokens only (0: all)")
+    p.add_argument("--top-p", type=float, default=1.0, help="draw from the likeliest tokens that make up this share of the probability")
+    p.add_argument("--min-p", type=float, default=0.0, help="draw from tokens at least this likely beside the likeliest one only")
+    p.add_argument("--n", type=int, default=1, help="continuations of every prompt (computed once; --seed counts up with them)")
+    p.add_argument("--logprobs", type=int, default=None, metavar="TOP", help="print the log-probability of every token, and the TOP likeliest ones")
     p.add_argument("--seed", type=int, default=None)
     p.add_argument("--eos-id", type=int, default=None)
     p.add_argument("--block-size", type=int, default=16, help="tokens per cache page")
@@ -56,7 +61,7 @@ def main(argv=None) -> int:
     p.add_argument("--config", default=None, help="a config.json for --random-weights")
     args = p.parse_args(argv)
 
-    from jax_vllm_b200 import (SamplingParams, add_request, has_work, load_from_path, make_driver, prewarm,
+    from jax_vllm_b200 import (SamplingParams, add_continuations, has_work, load_from_path, make_driver, prewarm,
                                random_model, registry, step)
 
     if args.random_weights is not None:
@@ -92,10 +97,10 @@ def main(argv=None) -> int:
         print(f"prewarm: done in {prewarm(driver):.1f}s", flush=True)
 
     sp = [SamplingParams(max_new_tokens=args.max_tokens, eos_id=args.eos_id, ignore_eos=args.ignore_eos,
-                         temperature=args.temperature,
-                         seed=None if args.seed is None else args.seed + i) for i in range(len(prompts))]
+                         temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p, logprobs=args.logprobs,
+                         seed=None if args.seed is None else args.seed + i * args.n) for i in range(len(prompts))]
     t0 = time.perf_counter()
-    ids = [add_request(driver, pr, s) for pr, s in zip(prompts, sp)]
+    ids = [i for pr, s in zip(prompts, sp) for i in add_continuations(driver, pr, args.n, s)]
     reqs = {i: driver.requests[i] for i in ids}
     while has_work(driver):
         step(driver)
@@ -106,7 +111,10 @@ def main(argv=None) -> int:
         n = len(r.output_ids)
         total += n
         ttft = (r.first_token_time - r.arrival) if r.first_token_time else 0.0
-        print(json.dumps({"request": i, "prompt_tokens": len(r.prompt_ids), "output_ids": r.output_ids}))
+        line = {"request": i, "prompt_tokens": len(r.prompt_ids), "output_ids": r.output_ids}
+        if args.logprobs is not None:
+            line.update(logprobs=r.logprobs, top_logprobs=r.top_logprobs)
+        print(json.dumps(line))
         if tokenizer is not None:
             print(tokenizer.decode(r.output_ids))
         print(f"  {n} tok · ttft {ttft:.3f}s", flush=True)

@@ -8,6 +8,10 @@ back when a request ends, when it is preempted, and - in a group with a window o
 chunks - as soon as every position of a page lies before what the next query can see (under a
 window that keeps the first tokens of a sequence, their pages stay).
 
+A request can be forked: the new one shares the full pages (they are never written again) and
+takes a copy of the last, partly filled page and of the state rows.  The pool can be resized: the
+pages in use move to the first pages of new stores (csrc/page_copy.cu makes both copies).
+
 Prefix reuse (jllm/engine/cache.py:20-57): full pages are hashed in a chain over the
 tokens; a new request takes the longest run of pages whose hashes are known, in every
 group, but always leaves at least its last token to compute.  A group with a window needs
@@ -26,6 +30,7 @@ from typing import Optional
 import numpy as np
 import torch
 
+from .. import ops
 from ..parts.base import FixedStateNeed, PagedKVNeed, PagedLayerCache, StateLayerCache
 from .page_pool import OutOfPages, PagePool, chain_hash
 from .state_slots import StateSlots
@@ -140,7 +145,9 @@ class CacheManager:
         self.slots = StateSlots(max_live)
         self.prefix_cache = bool(prefix_cache) and not self.state_layers
         self.live: dict[object, RequestCache] = {}
-        self.stats = {"prefix_hit_pages": 0, "prefix_hit_tokens": 0, "pages_allocated": 0, "pages_released": 0}
+        self.views: dict = {}                # what allocate_storage handed out, by (layer or (layer, member))
+        self.stats = {"prefix_hit_pages": 0, "prefix_hit_tokens": 0, "pages_allocated": 0, "pages_released": 0,
+                      "pages_shared": 0, "pages_copied": 0}
 
     # ------------------------------------------------------------------- storage
     def allocate_storage(self, dtype: torch.dtype, device) -> dict:
@@ -156,6 +163,7 @@ class CacheManager:
                 views[layer] = PagedLayerCache(group=g, k=grp.k[i], v=grp.v[i])
         for layer, need in self.state_layers.items():
             views[layer] = StateLayerCache(self.slots.add_layer(layer, need.shape, need.dtype, device))
+        self.views = dict(views)
         for layer, members in self.composite.items():
             views[layer] = tuple(views.pop((layer, j), None) for j in range(members))
         return views
@@ -284,6 +292,85 @@ class CacheManager:
             grp.pool.release(held)
             self.stats["pages_released"] += len(held)
         self.slots.give_back(rc.slot)
+
+    # --------------------------------------------------------------- forks and sizes
+    def fork(self, request_id, new_ids) -> list:
+        """New requests that hold what `request_id` holds: they share its full pages; the last, partly filled page and the
+        state rows are copied for each (on the current stream, behind the steps issued so far).  All or nothing."""
+        rc = self.live[request_id]
+        new_ids = list(new_ids)
+        if len(set(new_ids)) != len(new_ids) or any(n in self.live for n in new_ids):
+            raise KeyError(f"one of the requests {new_ids!r} is already live, or named twice")
+        P = self.page_size
+        full, rest = divmod(rc.num_tokens, P)
+        if len(new_ids) > self.slots.num_free:
+            raise RuntimeError(f"{len(new_ids)} forks need state slots, {self.slots.num_free} are free")
+        if rest and any(g.pool.num_free < len(new_ids) for g in self.groups):
+            raise OutOfPages(f"{len(new_ids)} forks need a page each")
+        copies = [[] for _ in self.groups]            # per group: pages that take over the partly filled one
+        forks = []
+        for new in new_ids:
+            child = RequestCache(new, self.slots.take(clear=False), [PageTable() for _ in self.groups], rc.num_tokens,
+                                 list(rc.hashes), list(rc.freed_upto), list(rc.tokens))
+            for g, grp in enumerate(self.groups):
+                for page in rc.tables[g][:full]:
+                    if page >= 0:
+                        grp.pool.touch(page)
+                        self.stats["pages_shared"] += 1
+                    child.tables[g].append(page)
+                if rest:
+                    page = grp.pool.alloc()
+                    child.tables[g].append(page)
+                    copies[g].append(page)
+                    self.stats["pages_allocated"] += 1
+            self.live[new] = child
+            forks.append(child)
+        for g, grp in enumerate(self.groups):
+            if copies[g] and grp.k is not None:
+                stores = [grp.k] if grp.v is grp.k else [grp.k, grp.v]
+                with torch.cuda.device(grp.k.device):
+                    ops.copy_pages(stores, [rc.tables[g][full]] * len(copies[g]), copies[g], tokens=[rest] * len(copies[g]))
+                self.stats["pages_copied"] += len(copies[g])
+        states = list(self.slots.tensors.values())
+        if states and forks:
+            with torch.cuda.device(states[0].device):
+                ops.copy_slots(states, [rc.slot] * len(forks), [c.slot for c in forks])
+        return forks
+
+    def resize(self, num_pages: int) -> None:
+        """Gives every group `num_pages` pages: what live requests hold, and as many of the pages kept for reuse as fit, move
+        to the first pages of new stores; the views that `allocate_storage` handed out follow.  One store at a time: the
+        old and the new one exist beside each other while their pages are copied."""
+        if num_pages < 1:
+            raise ValueError("a pool needs at least one page")
+        pools = [grp.pool.resized(num_pages) for grp in self.groups]      # raises before anything has changed
+        for g, (grp, (pool, moved)) in enumerate(zip(self.groups, pools)):
+            for name in ("k",) if grp.v is grp.k else ("k", "v"):
+                old = getattr(grp, name)
+                if old is None:
+                    continue
+                new = torch.zeros((old.shape[0], num_pages, *old.shape[2:]), dtype=old.dtype, device=old.device)
+                if moved:
+                    with torch.cuda.device(old.device):
+                        ops.copy_pages([old], list(moved), list(moved.values()), into=[new])
+                shared = grp.v is grp.k
+                setattr(grp, name, new)
+                if shared:
+                    grp.v = new
+                for i, layer in enumerate(grp.layers):
+                    view = self.views[layer]
+                    if name == "k":
+                        view.k = new[i]
+                    if name == "v" or shared:
+                        view.v = new[i]
+                del old
+            grp.pool = pool
+            for rc in self.live.values():
+                table = rc.tables[g]
+                for i, page in enumerate(table):
+                    if page >= 0:
+                        table[i] = moved[page]
+        self.num_pages = num_pages
 
     # -------------------------------------------------------------------- checks
     def check(self) -> None:

@@ -97,6 +97,27 @@ class PagePool:
             if self.ref[p] == 0:
                 self._append(p)
 
+    def resized(self, num_pages: int) -> tuple:
+        """(a pool of another size that holds what this one holds, old page -> new page).  Held pages come first, in the order
+        of their ids; free pages with a known content follow while there is room, the ones used last before the others."""
+        held = [p for p in range(self.num_pages) if self.ref[p] > 0]
+        if len(held) > num_pages:
+            raise OutOfPages(f"{len(held)} pages are held, {num_pages} is too few")
+        cached = [p for p in self.free_pages() if self.hash_of[p] is not None and self.page_of_hash.get(self.hash_of[p]) == p]
+        cached = cached[max(0, len(cached) - (num_pages - len(held))):]
+        moved = {p: i for i, p in enumerate(held + cached)}
+        pool = PagePool(num_pages)
+        for p, i in moved.items():
+            h = self.hash_of[p]
+            if h is not None and self.page_of_hash.get(h) == p:
+                pool.hash_of[i] = h
+                pool.page_of_hash[h] = i
+            pool.ref[i] = self.ref[p]
+            pool._unlink(i)
+        for p in cached:                          # behind the pages without content, in the order of their use
+            pool._append(moved[p])
+        return pool, moved
+
     # --------------------------------------------------------------------- hashes
     def register(self, p: int, h: bytes) -> None:
         """Records that page p holds the content hashed h; the first page to claim a hash

@@ -28,13 +28,15 @@ class StateSlots:
     def num_free(self) -> int:
         return len(self.free)
 
-    def take(self) -> int:
+    def take(self, clear: bool = True) -> int:
+        """A free slot, its rows cleared unless the caller writes them."""
         if not self.free:
             raise RuntimeError("no free state slot")
         s = self.free.pop()
         self.held.add(s)
-        for t in self.tensors.values():
-            t[s].zero_()
+        if clear:
+            for t in self.tensors.values():
+                t[s].zero_()
         return s
 
     def give_back(self, slot: int) -> None:

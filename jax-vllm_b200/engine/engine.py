@@ -4,6 +4,10 @@
 (max_num_seqs, max_model_len, max_prefill_len, block_size, num_blocks, dtype), token ids
 in and out.  `step` admits, runs ONE batch on the device (decoded tokens and prompt
 portions together) and returns the events of the tokens it produced.
+
+Beyond the reference's: `add_continuations` continues one prompt in several ways and computes it
+once, `fork_request` branches a request where it stands, `resize_cache` gives the pool of pages
+another size while requests live.
 """
 
 from __future__ import annotations
@@ -11,6 +15,7 @@ from __future__ import annotations
 import threading
 import time
 import weakref
+from dataclasses import replace
 from typing import Iterator, Optional
 
 import torch
@@ -83,24 +88,113 @@ def make_driver(model, max_num_seqs: int = 4, max_model_len: int = 2048, max_pre
     return Driver(model, cfg, runner=runner, sampler=sampler)
 
 
-def add_request(driver: Driver, prompt_ids, sampling: Optional[SamplingParams] = None) -> int:
-    driver.router.raise_if_failed()
-    sp = sampling or SamplingParams()
+def _checked_prompt(driver: Driver, prompt_ids) -> list:
     prompt = [int(t) for t in prompt_ids]
     vocab = driver.model.spec.vocab_size
     if any(t < 0 or t >= vocab for t in prompt):
         raise ValueError(f"prompt holds token ids outside [0, {vocab})")
-    driver.scheduler.validate(prompt, sp)
+    return prompt
+
+
+def _new_request(driver: Driver, prompt: list, sampling: SamplingParams) -> Request:
     with driver.id_lock:
         rid = driver.next_id
         driver.next_id += 1
-    req = Request(request_id=rid, prompt_ids=prompt, sampling=sp, arrival=time.perf_counter())
     driver.router.open(rid)
+    return Request(request_id=rid, prompt_ids=prompt, sampling=sampling, arrival=time.perf_counter())
+
+
+def add_request(driver: Driver, prompt_ids, sampling: Optional[SamplingParams] = None) -> int:
+    driver.router.raise_if_failed()
+    sp = sampling or SamplingParams()
+    prompt = _checked_prompt(driver, prompt_ids)
+    driver.scheduler.validate(prompt, sp)
+    req = _new_request(driver, prompt, sp)
     with driver.step_lock:
-        driver.requests[rid] = req
+        driver.requests[req.request_id] = req
         driver.scheduler.add(req)
     driver.router.wake()
-    return rid
+    return req.request_id
+
+
+def add_continuations(driver: Driver, prompt_ids, n: int, sampling=None) -> list:
+    """Adds `n` requests that continue the same prompt; returns their ids.  The prompt is computed once: when its last
+    token is done, every continuation draws its first token from the same logits, and all but the first take over the
+    prompt's pages (full ones shared, the last copied) and states.  One that finds no state slot then waits and is computed
+    by itself.  `sampling`: parameters for all (a seed s becomes s, s + 1, ...; without one each has its own) or one per
+    continuation."""
+    driver.router.raise_if_failed()
+    if n < 1:
+        raise ValueError("at least one continuation")
+    if sampling is None or isinstance(sampling, SamplingParams):
+        one = sampling or SamplingParams()
+        sampling = [replace(one, seed=None if one.seed is None else one.seed + i) for i in range(n)]
+    if len(sampling) != n:
+        raise ValueError("one set of sampling parameters for all continuations, or one for each")
+    prompt = _checked_prompt(driver, prompt_ids)
+    for sp in sampling:
+        driver.scheduler.validate(prompt, sp)
+    reqs = [_new_request(driver, prompt, sp) for sp in sampling]
+    reqs[0].followers = reqs[1:]
+    with driver.step_lock:
+        for req in reqs:
+            driver.requests[req.request_id] = req
+        driver.scheduler.add(reqs[0])
+    driver.router.wake()
+    return [req.request_id for req in reqs]
+
+
+def fork_request(driver: Driver, request_id: int, sampling: Optional[SamplingParams] = None) -> int:
+    """Adds a request that goes on from where an unfinished one stands; returns its id.  It shares the full pages that the
+    other holds and takes a copy of the last page and of the states; without a free slot or page it waits and is computed
+    again.  Its tokens so far are the other's, its events those that it produces itself; `max_new_tokens` counts both.
+    `sampling` defaults to the other's parameters, without a seed."""
+    driver.router.raise_if_failed()
+    with driver.step_lock:
+        parent = driver.requests.get(request_id)
+        if parent is None or parent.finished:
+            raise KeyError(f"request {request_id} is not running")
+        if any(parent in r.followers for r in driver.requests.values()):
+            raise ValueError(f"request {request_id} waits for the prompt that it continues")
+        sp = sampling if sampling is not None else replace(parent.sampling, seed=None)
+        if len(parent.output_ids) >= sp.max_new_tokens:
+            raise ValueError(f"the request has {len(parent.output_ids)} tokens already, max_new_tokens is {sp.max_new_tokens}")
+        driver.scheduler.validate(parent.prompt_ids, sp)
+        child = _new_request(driver, parent.prompt_ids, sp)
+        child.output_ids = list(parent.output_ids)
+        driver.requests[child.request_id] = child
+        driver.scheduler.fork(parent, [child])
+    driver.router.wake()
+    return child.request_id
+
+
+def resize_cache(driver: Driver, num_blocks: int) -> None:
+    """Gives the cache `num_blocks` pages: fewer to return device memory, more to serve more requests.  Live requests go on;
+    their pages, and the ones kept for reuse as far as they fit, move to the new pool.  Refused where a request that is not
+    finished could need more pages than there would be.  The captured decode steps are dropped and captured again when
+    they are next needed."""
+    driver.router.raise_if_failed()
+    with driver.step_lock:
+        cache, sched = driver.cache, driver.scheduler
+        if not cache.groups:
+            raise ValueError("the model keeps no pages")
+        for req in list(sched.running) + list(sched.waiting):
+            for r in [req] + req.followers:
+                need = -(-(len(r.prompt_ids) + r.sampling.max_new_tokens) // cache.page_size)
+                if need > num_blocks:
+                    raise ValueError(f"request {r.request_id} may need {need} pages, {num_blocks} were asked for")
+        held = max(cache.num_pages - g.pool.num_free for g in cache.groups)
+        if num_blocks < max(1, held):
+            raise ValueError(f"{held} pages are in use, {num_blocks} were asked for")
+        driver.ahead = None
+        if hasattr(driver.runner, "forget_graphs"):
+            driver.runner.forget_graphs()
+        cache.resize(num_blocks)
+        if torch.device(driver.config.device).type == "cuda":
+            torch.cuda.empty_cache()             # what the old stores held goes back to the device
+        sched.version += 1
+        driver.num_blocks = num_blocks
+        driver.stats.pages_total = num_blocks
 
 
 def has_work(driver: Driver) -> bool:
@@ -123,12 +217,21 @@ def _step_locked(driver: Driver) -> list:
     entries = [StepEntry(driver.cache.live[s.request.request_id], s.tokens, (len(s.tokens) - 1,) if s.wants_logits else ())
                for s in plan]
     sampled = [s for s in plan if s.wants_logits]
-    temps = [s.request.sampling.temperature for s in sampled]
-    seeds = [s.request.sampling.seed if s.request.sampling.seed is not None else s.request.request_id for s in sampled]
-    counters = [len(s.request.output_ids) for s in sampled]
+    # one draw for every request whose logits are there, and for every continuation that waits for its prompt
+    draws = [(row, req) for row, s in enumerate(sampled) for req in [s.request] + s.request.followers]
+    forking = len(draws) > len(sampled)
+    params = [req.sampling for _, req in draws]
+    temps = [sp.temperature for sp in params]
+    seeds = [sp.seed if sp.seed is not None else req.request_id for sp, (_, req) in zip(params, draws)]
+    counters = [len(req.output_ids) for _, req in draws]
+    filters = [(sp.top_k, sp.top_p, sp.min_p) if sp.filtered else (0, 1.0, 0.0) for sp in params] \
+        if any(sp.filtered for sp in params) else None
+    top = max([-1] + [sp.logprobs for sp in params if sp.logprobs is not None])      # -1: nobody wants log-probabilities
     # a decode-only step samples inside its replayed graph; any other step hands back logits for the sampler
     fused = getattr(driver.runner, "step_sampled", None)
-    both = fused(entries, temps, seeds, counters) if fused is not None and len(sampled) == len(plan) else None
+    more = () if filters is None else (filters,)
+    both = fused(entries, temps, seeds, counters, *more) \
+        if fused is not None and len(sampled) == len(plan) and not forking and top < 0 else None
     logits = driver.runner.step(entries) if both is None else None
     sched.committed(plan)
     st = driver.stats
@@ -143,8 +246,19 @@ def _step_locked(driver: Driver) -> list:
     if not sampled:
         return events
     if both is None:
-        tokens = driver.sampler.sample(logits, temps, seeds, counters)
-        both = torch.cat([tokens, driver.runner.status_word()])          # one copy back
+        if forking:
+            rows = [row for row, _ in draws]
+            logits = driver.sampler.repeat_rows(logits, rows) if logits.is_cuda else logits[rows]
+        if filters is None:
+            tokens = driver.sampler.sample(logits, temps, seeds, counters)
+        else:
+            tokens = driver.sampler.sample_filtered(logits, temps, seeds, counters, filters)
+        parts = [tokens, driver.runner.status_word()]
+        if top >= 0:
+            chosen, top_tokens, top_values = driver.sampler.logprobs(logits, tokens, top)
+            top = top_tokens.shape[1]
+            parts += [chosen.view(torch.int32), top_tokens.reshape(-1), top_values.view(torch.int32).reshape(-1)]
+        both = torch.cat(parts)                                          # one copy back
     arrived = None
     if both.is_cuda:
         # the copy is on its way while the host plans the next step; waiting for it also synchronises
@@ -155,31 +269,72 @@ def _step_locked(driver: Driver) -> list:
         arrived = torch.cuda.Event()
         arrived.record()
         both = back
-    driver.ahead = sched.plan_ahead(plan)
-    if driver.ahead is not None and fused is not None:
+    driver.ahead = sched.plan_ahead(plan) if not forking else None
+    if driver.ahead is not None and fused is not None and top < 0:
         # its layout goes into the staging buffer now too; only the tokens are missing
         driver.runner.prefill_ahead([StepEntry(driver.cache.live[s.request.request_id], [0], (0,)) for s in driver.ahead[1]],
-                                    temps, seeds, [c + 1 for c in counters])
+                                    temps, seeds, [c + 1 for c in counters], *more)
     if arrived is not None:
         arrived.synchronize()
-    both = both.tolist()
+    n = len(draws)
+    scores = likely = likely_scores = None
+    if top >= 0:
+        floats = both.view(torch.float32)
+        scores = floats[n + 1:2 * n + 1].tolist()
+        likely = both[2 * n + 1:2 * n + 1 + n * top].tolist()
+        likely_scores = floats[2 * n + 1 + n * top:].tolist()
+    both = both[:n + 1].tolist()
     toks, status = both[:-1], both[-1]
     if status:
         driver.runner.clear_status()
         from ..ops import raise_on_status
         raise_on_status(status)
     now = time.perf_counter()
-    for s, tok in zip(sampled, toks):
-        req = s.request
-        req.output_ids.append(int(tok))
+    by_row = [[] for _ in sampled]
+    for k, ((row, req), tok) in enumerate(zip(draws, toks)):
+        event = StepEvent(req.request_id, int(tok), False)
+        if req.sampling.logprobs is not None:
+            m = min(req.sampling.logprobs, top)
+            event.logprob = scores[k]
+            event.top_logprobs = list(zip(likely[k * top:k * top + m], likely_scores[k * top:k * top + m]))
+            req.logprobs.append(event.logprob)
+            req.top_logprobs.append(event.top_logprobs)
+        req.output_ids.append(event.token)
         if req.first_token_time is None:
             req.first_token_time = now
         driver.stats.emitted_tokens += 1
-        done = len(req.output_ids) >= req.sampling.max_new_tokens or req.sampling.stops_at(int(tok))
-        if done:
-            sched.finish(req)
-        events.append(StepEvent(req.request_id, int(tok), done))
+        event.finished = len(req.output_ids) >= req.sampling.max_new_tokens or req.sampling.stops_at(event.token)
+        by_row[row].append((req, event))
+        events.append(event)
+    for s, made in zip(sampled, by_row):
+        # continuations go on from what the first of them holds, before it may be given back
+        go_on = [req for req, event in made[1:] if not event.finished]
+        for req, event in made[1:]:
+            if event.finished:
+                sched.finish_unstarted(req)
+        s.request.followers = []
+        if go_on:
+            sched.fork(s.request, go_on)
+        if made[0][1].finished:
+            sched.finish(s.request)
     return events
+
+
+def _run_to_end(driver: Driver, ids: list) -> list:
+    reqs = [driver.requests[i] for i in ids]
+    while any(not r.finished for r in reqs):
+        if not step(driver) and not has_work(driver):
+            break
+    for i in ids:
+        driver.router.close(i)
+        driver.requests.pop(i, None)
+    return reqs
+
+
+def continuations(driver: Driver, prompt_ids, n: int, sampling=None) -> list:
+    """Runs `n` continuations of a prompt to completion (see `add_continuations`); returns their Request records, with
+    `output_ids` and, where they were asked for, `logprobs`: the likeliest one is max(..., key=lambda r: sum(r.logprobs))."""
+    return _run_to_end(driver, add_continuations(driver, prompt_ids, n, sampling))
 
 
 def generate(driver: Driver, prompts, sampling=None) -> list:
@@ -188,14 +343,7 @@ def generate(driver: Driver, prompts, sampling=None) -> list:
     if sampling is None or isinstance(sampling, SamplingParams):
         sampling = [sampling] * len(prompts)
     ids = [add_request(driver, p, sp) for p, sp in zip(prompts, sampling)]
-    reqs = [driver.requests[i] for i in ids]
-    while any(not r.finished for r in reqs):
-        if not step(driver) and not has_work(driver):
-            break
-    for i in ids:
-        driver.router.close(i)
-        driver.requests.pop(i, None)
-    return [list(r.output_ids) for r in reqs]
+    return [list(r.output_ids) for r in _run_to_end(driver, ids)]
 
 
 # --------------------------------------------------------------- streams and thread

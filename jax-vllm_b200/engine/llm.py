@@ -20,8 +20,20 @@ class LLM:
     def generate(self, prompts, sampling: SamplingParams | list | None = None) -> list:
         return eng.generate(self.driver, prompts, sampling)
 
+    def continuations(self, prompt_ids, n: int, sampling: SamplingParams | list | None = None) -> list:
+        return eng.continuations(self.driver, prompt_ids, n, sampling)
+
     def add_request(self, prompt_ids, sampling=None) -> int:
         return eng.add_request(self.driver, prompt_ids, sampling)
+
+    def add_continuations(self, prompt_ids, n: int, sampling=None) -> list:
+        return eng.add_continuations(self.driver, prompt_ids, n, sampling)
+
+    def fork_request(self, request_id: int, sampling: SamplingParams | None = None) -> int:
+        return eng.fork_request(self.driver, request_id, sampling)
+
+    def resize_cache(self, num_blocks: int) -> None:
+        eng.resize_cache(self.driver, num_blocks)
 
     def step(self):
         return eng.step(self.driver)

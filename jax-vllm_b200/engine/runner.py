@@ -39,12 +39,12 @@ class _DecodeGraph:
     """A captured step for `n` single-token entries: fixed buffers, fixed launch sizes.  With sampling in
     the graph, `out` holds the sampled tokens followed by the kernels' status word, and the sampling
     parameters lie behind the batch in the same buffer, from `samp_off` on: n seeds and n counters (64-bit),
-    then n temperatures."""
+    then n temperatures and, with filters, n numbers each for top_k, top_p and min_p."""
 
-    def __init__(self, layout, dev, logits, graph, launches, out=None, samp_off=0):
+    def __init__(self, layout, dev, logits, graph, launches, out=None, samp_off=0, filtered=False):
         self.layout, self.dev, self.logits, self.graph, self.launches = layout, dev, logits, graph, launches
         self.out, self.samp_off = out, samp_off
-        self.total = layout.total if out is None else samp_off + 5 * layout.sections["token_ids"][1]
+        self.total = layout.total if out is None else samp_off + (8 if filtered else 5) * layout.sections["token_ids"][1]
 
 
 class Runner:
@@ -64,6 +64,7 @@ class Runner:
         # all batch sizes together hold what the largest needs, not the sum.
         self.graph_pool = None
         self.graphs_sampled: dict[int, _DecodeGraph] = {}
+        self.graphs_filtered: dict[int, _DecodeGraph] = {}
         self.graph_warm: set[int] = set()
         self._ahead = None                 # (requests and lengths, graph) of a batch already laid out in the staging buffer
         self.launches_last_step = 0
@@ -74,7 +75,7 @@ class Runner:
         self.device, self.dtype = torch.device(device), dtype
         if self.device.type != "cuda":
             raise RuntimeError("the engine runs on a CUDA device only (there is no CPU path)")
-        kernel_build.build_all(model.kernels() + ["sampling"])
+        kernel_build.build_all(model.kernels() + ["sampling", "sample_filtered", "token_logprobs", "page_copy"])
         views = cache.allocate_storage(dtype, self.device)
         self.layer_caches = [views.get(k) for k in range(len(model.order))]
         self.builder = BatchBuilder(len(cache.groups), cache.page_size, model.tile_classes(cache.page_size), self.device)
@@ -155,55 +156,78 @@ class Runner:
         ops.launch_count += g.launches
         return g.logits
 
+    def forget_graphs(self) -> None:
+        """Drops every captured step (the cache is about to move).  They are captured again when they are next needed."""
+        torch.cuda.synchronize(self.device)
+        self._ahead = None
+        self.graphs.clear(); self.graphs_sampled.clear(); self.graphs_filtered.clear()
+        self.graph_pool = None
+
     # ------------------------------------------- captured decode steps that also sample
     @staticmethod
     def _key(entries):
         return tuple((e.cache.request_id, e.cache.num_tokens) for e in entries)
 
-    def _fill_sampling(self, host, g: _DecodeGraph, temps, seeds, counters) -> None:
+    def _fill_sampling(self, host, g: _DecodeGraph, temps, seeds, counters, filters=None) -> None:
         n = len(temps)
         wide = host[g.samp_off:g.samp_off + 4 * n].view("int64")
         wide[:n] = [s & ((1 << 63) - 1) for s in seeds]
         wide[n:2 * n] = counters
         host[g.samp_off + 4 * n:g.samp_off + 5 * n].view("float32")[:] = temps
+        if filters is not None:
+            top_k, top_p, min_p = zip(*filters)
+            host[g.samp_off + 5 * n:g.samp_off + 6 * n] = top_k
+            host[g.samp_off + 6 * n:g.samp_off + 7 * n].view("float32")[:] = top_p
+            host[g.samp_off + 7 * n:g.samp_off + 8 * n].view("float32")[:] = min_p
 
     @torch.no_grad()
-    def step_sampled(self, entries: list, temps, seeds, counters):
+    def step_sampled(self, entries: list, temps, seeds, counters, filters=None):
         """A decode-only step with the sampling inside the replayed graph: returns the sampled tokens followed
         by the kernels' status word (int32, on the device), or None if this batch has to go the ordinary way
-        (`step`, then the sampler): not all single tokens, or the first time at this batch size."""
+        (`step`, then the sampler): not all single tokens, or the first time at this batch size.  `filters`: None, or
+        (top_k, top_p, min_p) of every entry, for which there is a graph of its own."""
         n = len(entries)
         if not self._graphable(entries) or n not in self.graph_warm:
             return None
         b = self.builder
         with torch.cuda.device(self.device):
-            g = self.graphs_sampled.get(n)
+            graphs = self.graphs_sampled if filters is None else self.graphs_filtered
+            g = graphs.get(n)
             if g is None:
                 layout = self._graph_layout(entries)
                 samp_off = (layout.total + 1) // 2 * 2
-                dev = torch.zeros(samp_off + 5 * n, dtype=torch.int32, device=self.device)
+                dev = torch.zeros(samp_off + (5 if filters is None else 8) * n, dtype=torch.int32, device=self.device)
                 out = torch.zeros(n + 1, dtype=torch.int32, device=self.device)
-                g = _DecodeGraph(layout, dev, None, None, 0, out=out, samp_off=samp_off)
+                g = _DecodeGraph(layout, dev, None, None, 0, out=out, samp_off=samp_off, filtered=filters is not None)
                 pinned = b._staging(g.total)
                 host = pinned.numpy()[:g.total]
                 b.fill(entries, host, layout)
-                self._fill_sampling(host, g, temps, seeds, counters)
+                self._fill_sampling(host, g, temps, seeds, counters, filters)
                 dev.copy_(pinned[:g.total], non_blocking=True)
                 torch.cuda.current_stream().synchronize()
                 ctx = b.context(entries, layout, dev, max_seq_len=self.max_model_len)
                 seeds_d = dev[samp_off:samp_off + 2 * n].view(torch.int64)
                 counters_d = dev[samp_off + 2 * n:samp_off + 4 * n].view(torch.int64)
                 temps_d = dev[samp_off + 4 * n:samp_off + 5 * n].view(torch.float32)
+                if filters is not None:
+                    k_d, p_d, m_d = (dev[samp_off + k * n:samp_off + (k + 1) * n] for k in (5, 6, 7))
+                    # its one-time set-up outside the capture
+                    ops.sample_filtered(torch.zeros((n, self.model.spec.vocab_size), dtype=torch.float32, device=self.device), temps_d,
+                                        k_d, p_d.view(torch.float32), m_d.view(torch.float32), seeds_d, counters_d)
                 graph = torch.cuda.CUDAGraph()
                 before = ops.launch_count
                 with _capture(graph, self._pool()):
                     logits = self.model.forward(ctx, self.layer_caches)
-                    out[:n].copy_(ops.sample(logits, temps_d, seeds_d, counters_d))
+                    if filters is None:
+                        tokens = ops.sample(logits, temps_d, seeds_d, counters_d)
+                    else:
+                        tokens = ops.sample_filtered(logits, temps_d, k_d, p_d.view(torch.float32), m_d.view(torch.float32), seeds_d, counters_d)
+                    out[:n].copy_(tokens)
                     out[n:].copy_(ops.status_word(self.device))
-                    del logits                  # only `out` is read after a replay: the logits' memory serves later captures
+                    del logits, tokens          # only `out` is read after a replay: the logits' memory serves later captures
                 g.graph, g.launches = graph, ops.launch_count - before
                 ops.launch_count = before       # nothing ran yet: a replay counts them
-                self.graphs_sampled[n] = g
+                graphs[n] = g
                 self._ahead = None
             ahead, self._ahead = self._ahead, None
             pinned = b._pinned
@@ -215,7 +239,7 @@ class Runner:
                 pinned = b._staging(g.total)
                 host = pinned.numpy()[:g.total]
                 b.fill(entries, host, g.layout)
-                self._fill_sampling(host, g, temps, seeds, counters)
+                self._fill_sampling(host, g, temps, seeds, counters, filters)
             g.dev.copy_(pinned[:g.total], non_blocking=True)
             b._copied = torch.cuda.Event(); b._copied.record()
             g.graph.replay()
@@ -224,19 +248,19 @@ class Runner:
         self.steps += 1
         return g.out
 
-    def prefill_ahead(self, entries: list, temps, seeds, counters) -> None:
+    def prefill_ahead(self, entries: list, temps, seeds, counters, filters=None) -> None:
         """Lays out the next decode step (tokens not known yet) in the staging buffer while the device runs
         this one.  `entries` carry the lengths that the requests will have then; `step_sampled` uses the
         layout if it is called with exactly these requests at these lengths."""
         self._ahead = None
-        g = self.graphs_sampled.get(len(entries))
+        g = (self.graphs_sampled if filters is None else self.graphs_filtered).get(len(entries))
         if g is None or not self._graphable(entries):
             return
         b = self.builder
         pinned = b._staging(g.total)          # waits until the last copy out of it has finished
         host = pinned.numpy()[:g.total]
         b.fill(entries, host, g.layout)
-        self._fill_sampling(host, g, temps, seeds, counters)
+        self._fill_sampling(host, g, temps, seeds, counters, filters)
         self._ahead = (self._key(entries), g)
 
     def run(self, entries: list) -> torch.Tensor:

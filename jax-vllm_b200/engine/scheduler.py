@@ -15,6 +15,8 @@ request - its pages and slot are given back, it returns to the front of the queu
 it is later run again over its prompt and the tokens it had generated (recomputation;
 with prefix reuse most of it is a cache hit).  A request that could never fit
 (prompt + max_new_tokens beyond the pool or max_model_len) is refused when it is added.
+A request can be forked (`fork`): the new one runs beside it from what it holds in the cache if a
+slot and a page are free, and else waits in the queue and is computed from its tokens.
 The reference never gets there: it refuses any pool smaller than the worst case
 (jllm/engine/engine.py:85-94); its order of work is admit, prefill, decode
 (jllm/engine/engine.py:161-168).
@@ -200,6 +202,29 @@ class Scheduler:
             s.tokens = [s.request.output_ids[-1]]        # pending == 1: the token sampled last
         self.stats.scheduler_loops += 1
         return plan
+
+    def fork(self, parent: Request, children: list) -> None:
+        """Requests that start from `parent`'s tokens.  Those that find a slot and a page run from what it holds in the cache;
+        the others wait at the front of the queue (where `parent` itself does not run: all of them, at its end)."""
+        self.version += 1
+        if parent.request_id not in self.cache.live:
+            self.waiting.extend(children)
+            return
+        fits = self.cache.slots.num_free
+        if self.cache.live[parent.request_id].num_tokens % self.cache.page_size:
+            fits = min([fits] + [g.pool.num_free for g in self.cache.groups])
+        run, wait = children[:fits], children[fits:]
+        if run:
+            for child, rc in zip(run, self.cache.fork(parent.request_id, [c.request_id for c in run])):
+                child.slot = rc.slot
+                self.running.append(child)
+            self.stats.forks += len(run)
+        self.waiting.extendleft(reversed(wait))
+
+    def finish_unstarted(self, req: Request) -> None:
+        """A request that ends before it held anything: a continuation whose first token is its last."""
+        req.finished = True
+        self.stats.finished += 1
 
     def finish(self, req: Request) -> None:
         self.version += 1

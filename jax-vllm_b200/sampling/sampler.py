@@ -1,4 +1,5 @@
-"""Greedy and temperature sampling on the device (csrc/sampling.cu).
+"""Greedy, temperature and filtered sampling on the device (csrc/sampling.cu, csrc/sample_filtered.cu), and the
+log-probabilities of what was sampled (csrc/token_logprobs.cu).
 
 The reference samples greedily only (argmax, jllm/engine/generate.py:142 and
 jllm/engine/state.py:66).  Temperature sampling here is a draw from
@@ -45,6 +46,26 @@ class Sampler:
         sc = torch.tensor([[s & ((1 << 63) - 1) for s in seeds], list(counters)], dtype=torch.int64)
         sc = sc.to(self.device, non_blocking=True)
         return ops.sample(logits, t, sc[0].contiguous(), sc[1].contiguous())
+
+    def sample_filtered(self, logits: torch.Tensor, temperatures, seeds, counters, filters) -> torch.Tensor:
+        """The same under filters: (top_k, top_p, min_p) per row.  A row whose filters are off gets the token of `sample`."""
+        rows = logits.shape[0]
+        if not (len(temperatures) == len(seeds) == len(counters) == len(filters) == rows):
+            raise ValueError("one temperature, seed, counter and set of filters per row of logits")
+        top_k, top_p, min_p = zip(*filters)
+        f = torch.tensor([list(temperatures), top_p, min_p], dtype=torch.float32).to(self.device, non_blocking=True)
+        k = torch.tensor(top_k, dtype=torch.int32).to(self.device, non_blocking=True)
+        sc = torch.tensor([[s & ((1 << 63) - 1) for s in seeds], list(counters)], dtype=torch.int64)
+        sc = sc.to(self.device, non_blocking=True)
+        return ops.sample_filtered(logits, f[0], k, f[1], f[2], sc[0], sc[1])
+
+    def logprobs(self, logits: torch.Tensor, tokens: torch.Tensor, top: int) -> tuple:
+        """(log-probability of each row's token, the `top` likeliest tokens, theirs), on the device."""
+        return ops.token_logprobs(logits, tokens, min(top, logits.shape[1]))
+
+    def repeat_rows(self, logits: torch.Tensor, rows: list) -> torch.Tensor:
+        """The logits of the given rows, in that order."""
+        return ops.embed_gather(logits, torch.tensor(rows, dtype=torch.int32).to(self.device, non_blocking=True))
 
     def greedy(self, logits: torch.Tensor) -> torch.Tensor:
         rows = logits.shape[0]
