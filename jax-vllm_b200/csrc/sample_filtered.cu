@@ -42,14 +42,13 @@ struct Scores {
   float temp, per;                                     // T and log2(e) / T
   u64 base;
 
-  __device__ __forceinline__ u64 bits(int i) const { return jv_draw_bits(base, (u64)i); }
-  __device__ __forceinline__ float of(float x, u64 bits) const {
-    return x / temp - logf(-logf(((float)(unsigned)(bits >> 40) + 0.5f) * (1.0f / 16777216.0f)));
+  __device__ __forceinline__ float of(float x, int i) const {
+    return x / temp - logf(-logf(((float)(unsigned)(jv_draw_bits(base, (unsigned)i) >> 40) + 0.5f) * (1.0f / 16777216.0f)));
   }
-  // Whether the score may reach `enough` (given as enough * log2(e)), but for roundings: -log(-log(u)) <= -log(1 - u), and
-  // 1 - u is no less than what the first 23 random bits leave of it.
-  __device__ __forceinline__ bool may_reach(float x, u64 bits, float enough2) const {
-    const float w = (2.f - 1.1920929e-7f) - __uint_as_float(0x3f800000u | (unsigned)(bits >> 41));
+  // Whether the score of token i may reach `enough` (given as enough * log2(e)), but for roundings: -log(-log(u)) <= -log(1 - u),
+  // and 1 - u is no less than what the first 23 random bits leave of it.
+  __device__ __forceinline__ bool may_reach(float x, int i, float enough2) const {
+    const float w = (2.f - 1.1920929e-7f) - __uint_as_float(0x3f800000u | jv_draw_first23(base, (unsigned)i));
     return !(w > exp2_fast(fmaf(x, per, -enough2)));
   }
 };
@@ -69,17 +68,16 @@ struct Draw {
     if (!__any_sync(0xffffffffu, which != 0)) return;
     unsigned may = 0;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) may |= sc.may_reach(x[i], sc.bits(at + i), enough2) ? 1u << i : 0u;
+    for (int i = 0; i < VEC; ++i) may |= sc.may_reach(x[i], at + i, enough2) ? 1u << i : 0u;
     may &= which;
     for (unsigned left = __reduce_or_sync(0xffffffffu, may); left; left &= left - 1) {
       const int i = __ffs(left) - 1;
       float y = x[0];
 #pragma unroll
       for (int k = 1; k < VEC; ++k) y = i == k ? x[k] : y;
-      const u64 bits = sc.bits(at + i);
-      const bool still = (may >> i & 1) && sc.may_reach(y, bits, enough2);
+      const bool still = (may >> i & 1) && sc.may_reach(y, at + i, enough2);
       if (!__any_sync(0xffffffffu, still)) continue;
-      if (still) take_better(best.v, best.i, sc.of(y, bits), at + i);
+      if (still) take_better(best.v, best.i, sc.of(y, at + i), at + i);
       const unsigned known = __reduce_max_sync(0xffffffffu, key_of(best.v));
       unsigned of_block = known;
       if ((threadIdx.x & 31) == 0) of_block = max(known, atomicMax(&shared().best_key, known));
@@ -117,8 +115,7 @@ template <typename T> __device__ __noinline__ Best largest_of_row() {
   Best best{-INFINITY, 0x7fffffff};
   each<T, 8>([&](const auto& x, int at) {
 #pragma unroll
-    for (int i = 0; i < 16 / (int)sizeof(T); ++i)
-      if (x[i] > best.v) best = Best{x[i], at + i};    // a thread's tokens come in the order of their indices
+    for (int i = 0; i < 16 / (int)sizeof(T); ++i) take_better(best.v, best.i, x[i], at + i);
   });
   return best;
 }
@@ -355,7 +352,7 @@ __global__ void __launch_bounds__(NT, 2) sample_filtered_kernel(const SamplePara
     best = Best{-INFINITY, 0x7fffffff};
     for (int i = threadIdx.x; i < listed; i += NT) {
       const u64 c = sh.list[i];
-      take_better(best.v, best.i, sc.of(logit_of(c), sc.bits(index_of(c))), index_of(c));
+      take_better(best.v, best.i, sc.of(logit_of(c), index_of(c)), index_of(c));
     }
     block_best(best.v, best.i, sh.warp_v, sh.warp_i);
   }

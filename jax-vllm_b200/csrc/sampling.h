@@ -19,6 +19,14 @@ __host__ __device__ __forceinline__ unsigned long long jv_draw_bits(unsigned lon
   return jv_mix64(base ^ (v * 0xD1342543DE82EF95ULL + 0x2545F4914F6CDD1DULL));
 }
 
+// The first 23 of them.  (The last shift of jv_mix64 reaches none but the lowest of the high word's bits.)
+__host__ __device__ __forceinline__ unsigned jv_draw_first23(unsigned long long base, unsigned long long v) {
+  unsigned long long z = base ^ (v * 0xD1342543DE82EF95ULL + 0x2545F4914F6CDD1DULL);
+  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ULL;
+  z = (z ^ (z >> 27)) * 0x94D049BB133111EBULL;
+  return (unsigned)(z >> 41);
+}
+
 // Uniform in (0, 1) with 24 random bits.
 __host__ __device__ __forceinline__ float jv_uniform(unsigned long long seed, unsigned long long counter,
                                                      unsigned long long v) {

@@ -101,10 +101,9 @@ struct Shared {
   double warp_d[2][WARPS];
   float warp_v[32];
   int warp_i[32];
-  // the row: vectors of sixteen bytes that start on sixteen-byte boundaries, `off` elements of the first before the row; those
-  // from `whole` to `ragged` lie in it with all their elements
+  // the row: `vectors` of sixteen bytes from the first sixteen-byte boundary on, `head` elements before them, some behind
   const void* row;
-  int n, off, vectors, whole, ragged, blocks, rank, parity;
+  int n, head, vectors, blocks, rank, parity;
   float largest, scale, bound;                         // bound: at least `j * blocks` tokens are no smaller; scale: log2(e) / T
   Range range;
   u64 told;                                            // the boundary, from the first block
@@ -161,10 +160,8 @@ template <typename T> __device__ __forceinline__ void begin(const T* row, int n,
     const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     sh.row = row;
     sh.n = n;
-    sh.off = off;
-    sh.vectors = (off + n + VEC - 1) / VEC;
-    sh.whole = off == 0 ? 0 : 1;
-    sh.ragged = (off + n) / VEC;
+    sh.head = min(n, (VEC - off) % VEC);
+    sh.vectors = (n - sh.head) / VEC;
     sh.blocks = blocks;
     sh.rank = blocks > 1 ? (int)cg::this_cluster().block_rank() : 0;
     sh.parity = 0;
@@ -188,69 +185,62 @@ template <typename V> __device__ __forceinline__ V* of(V* mine, int b) {
 }
 
 // ---------------------------------------------------------------------------------------------------------- passes
-// Sixteen bytes of the row of which some lie outside it: those read as NaN.
-template <typename T> __device__ __noinline__ uint4 load_part(const T* row, int at, int n) {
+// The elements before the first vector and behind the last one, as two vectors that read as NaN elsewhere: `which` 0 or 1.
+template <typename T> __device__ __forceinline__ int first_of_end(int which) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  return which == 0 ? shared().head - VEC : shared().head + shared().vectors * VEC;
+}
+template <typename T> __device__ __noinline__ uint4 load_end(int which) {
+  const Shared& sh = shared();
+  const T* row = reinterpret_cast<const T*>(sh.row);
+  const int at = first_of_end<T>(which), from = which == 0 ? 0 : at, to = which == 0 ? sh.head : sh.n;
   unsigned w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (sizeof(T) == 4) {
-      w[i] = at + i >= 0 && at + i < n ? reinterpret_cast<const unsigned*>(row)[at + i] : 0x7fffffffu;
+      w[i] = at + i >= from && at + i < to ? reinterpret_cast<const unsigned*>(row)[at + i] : 0x7fffffffu;
     } else {
       const int l = at + 2 * i, h = l + 1;
-      w[i] = (l >= 0 && l < n ? reinterpret_cast<const unsigned short*>(row)[l] : 0x7fffu) |
-             (h >= 0 && h < n ? (unsigned)reinterpret_cast<const unsigned short*>(row)[h] : 0x7fffu) << 16;
+      w[i] = (l >= from && l < to ? reinterpret_cast<const unsigned short*>(row)[l] : 0x7fffu) |
+             (h >= from && h < to ? (unsigned)reinterpret_cast<const unsigned short*>(row)[h] : 0x7fffu) << 16;
     }
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+__device__ __forceinline__ uint4 no_vector() { return make_uint4(0x7fffffffu, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu); }   // NaNs of either type
 
-// The vectors of the row that a thread reads one after the other: j, j + step, ...
-template <typename T> struct Vectors {
-  static constexpr int VEC = 16 / (int)sizeof(T);
-  const T* row;
-  int n, off, count, whole, ragged, step, start;
-
-  __device__ __forceinline__ Vectors() {
-    const Shared& sh = shared();
-    row = reinterpret_cast<const T*>(sh.row);
-    n = sh.n; off = sh.off; count = sh.vectors; whole = sh.whole; ragged = sh.ragged;
-    step = sh.blocks * NT;
-    start = sh.rank * NT + threadIdx.x;
-  }
-  __device__ __forceinline__ int first(int j) const { return j * VEC - off; }
-  // AHEAD of them from j on: all are asked for before the few that lie in the row in part.  NaNs where there is none.
-  template <int AHEAD> __device__ __forceinline__ void load(int j, uint4 (&raw)[AHEAD]) const {
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int k = j + u * step;
-      raw[u] = make_uint4(0x7fffffffu, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu);
-      if (k >= whole && k < ragged) raw[u] = *reinterpret_cast<const uint4*>(row + first(k));
-    }
-    if (j < whole || (j + (AHEAD - 1) * step >= ragged && ragged < count)) {
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const int k = j + u * step;
-        if (k < count && !(k >= whole && k < ragged)) raw[u] = load_part(row, first(k), n);
-      }
-    }
-  }
-};
-
-// f(values, index of the first) for the vectors that this thread reads, AHEAD loads before the first is used; what lies outside
-// the row is NaN.  With WHOLE the lanes of a warp come together for every vector: those with none left get NaNs.
+// f(values, index of the first) for the vectors that this thread reads, AHEAD loads before the first is used, and then for the
+// ends of the row; what lies outside the row is NaN.  With WHOLE the lanes of a warp come together for every vector: those
+// with none left get NaNs.
 template <typename T, int AHEAD, bool WHOLE = false, typename F> __device__ __forceinline__ void each(F&& f) {
-  const Vectors<T> v;
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const Shared& sh = shared();
+  const int step = sh.blocks * NT, start = sh.rank * NT + threadIdx.x, vectors = sh.vectors;
   const int lane = WHOLE ? threadIdx.x & 31 : 0;
-  for (int j = v.start; j - lane < v.count; j += AHEAD * v.step) {
-    uint4 raw[AHEAD];
-    v.template load<AHEAD>(j, raw);
+  {
+    const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(sh.row) + sh.head) + start;
+    int at = sh.head + start * VEC;
+    for (int left = vectors - start; left + lane > 0; left -= AHEAD * step) {
+      uint4 raw[AHEAD];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-      if (j - lane + u * v.step < v.count) {
-        float x[Vectors<T>::VEC];
-        unpack<T>(raw[u], x);
-        f(x, v.first(j + u * v.step));
-      }
+      for (int u = 0; u < AHEAD; ++u)
+        if (left > u * step) raw[u] = p[u * step];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (left + lane > u * step) {
+          float x[VEC];
+          if (WHOLE && left <= u * step) raw[u] = no_vector();
+          unpack<T>(raw[u], x);
+          f(x, at + u * step * VEC);
+        }
+      p += AHEAD * step;
+      at += AHEAD * step * VEC;
+    }
+  }
+  if (start - lane < 2) {                              // the row's first two threads (with WHOLE: their warp)
+    float x[VEC];
+    unpack<T>(start < 2 ? load_end<T>(start) : no_vector(), x);
+    f(x, first_of_end<T>(start));
   }
 }
 
@@ -383,49 +373,62 @@ static __device__ __noinline__ unsigned send_list() {
 // infinity is not put, nor what lies more than `deepest` below the largest.  Returns this thread's largest logit and, SUMMED,
 // the sum of its masses, relative to that one's.
 template <typename T, bool SUMMED> __device__ __noinline__ float2 put_once(int j, float deepest) {
-  constexpr int AHEAD = 4;
-  const Vectors<T> v;
+  constexpr int VEC = 16 / (int)sizeof(T), AHEAD = 4;
   const float scale = shared().scale;
+  const int vectors = shared().vectors;
   float m = -INFINITY, s = 0.f, least = INFINITY;
-  const int rounds = (v.count + AHEAD * NT - 1) / (AHEAD * NT);
-  for (int k = 0; k < rounds; ++k) {
-    const int first = k * AHEAD * NT + threadIdx.x;
+  const auto take = [&](const uint4& raw, int at) {
+    float x[VEC];
+    unpack<T>(raw, x);
+    float big = x[0];                                  // (a NaN is passed over)
+#pragma unroll
+    for (int i = 1; i < VEC; ++i) big = fmaxf(big, x[i]);
+    if (SUMMED) {
+      if (big > m) s *= exp2_fast(-(fminf(big - m, HUGE_F) * scale));
+      const float to = fmaxf(big, m);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s += x[i] > -INFINITY ? exp2_fast(-(below(x[i], to) * scale)) : 0.f;
+    }
+    m = fmaxf(m, big);
+    if (big >= least) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (x[i] >= least) put(compose(clean(x[i]), at + i));
+    }
+  };
+  const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(shared().row) + shared().head) + threadIdx.x;
+  int at = shared().head + threadIdx.x * VEC;
+  uint4 next[AHEAD];                                   // the loads of the round to come are on their way during one
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) next[u] = (int)threadIdx.x + u * NT < vectors ? p[u * NT] : no_vector();
+  for (int k = 0; k == 0 || k * AHEAD * NT < vectors; ++k) {
     uint4 raw[AHEAD];
-    v.template load<AHEAD>(first, raw);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) raw[u] = next[u];
+    p += AHEAD * NT;
+    const int left = vectors - (k + 1) * AHEAD * NT - (int)threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) next[u] = left > u * NT ? p[u * NT] : no_vector();
     if (k == 0 || k == 3) {                            // what the first vectors hold above their own bound
       float g = m;
       if (k == 0) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-          float x[v.VEC];
+          float x[VEC];
           unpack<T>(raw[u], x);
 #pragma unroll
-          for (int i = 0; i < v.VEC; ++i) g = fmaxf(g, x[i]);
+          for (int i = 0; i < VEC; ++i) g = fmaxf(g, x[i]);
         }
       }
       exchange_largest(g, j);
       least = fmaxf(fmaxf(shared().bound, -HUGE_F), shared().largest - deepest);
     }
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      float x[v.VEC];
-      unpack<T>(raw[u], x);
-      float big = x[0];                                // (a NaN is passed over)
-#pragma unroll
-      for (int i = 1; i < v.VEC; ++i) big = fmaxf(big, x[i]);
-      if (SUMMED) {
-        if (big > m) s *= exp2_fast(-(fminf(big - m, HUGE_F) * scale));
-        const float to = fmaxf(big, m);
-#pragma unroll
-        for (int i = 0; i < v.VEC; ++i) s += x[i] > -INFINITY ? exp2_fast(-(below(x[i], to) * scale)) : 0.f;
-      }
-      m = fmaxf(m, big);
-      if (big >= least) {
-#pragma unroll
-        for (int i = 0; i < v.VEC; ++i)
-          if (x[i] >= least) put(compose(clean(x[i]), v.first(first + u * NT) + i));
-      }
-    }
+    for (int u = 0; u < AHEAD; ++u) take(raw[u], at + u * NT * VEC);
+    at += AHEAD * NT * VEC;
+  }
+  if (threadIdx.x < 2) {
+    take(load_end<T>(threadIdx.x), first_of_end<T>(threadIdx.x));
   }
   return make_float2(m, s);
 }
