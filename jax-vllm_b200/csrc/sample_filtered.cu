@@ -63,21 +63,24 @@ struct Draw {
   float enough2 = -INFINITY;
 
   __device__ __forceinline__ Draw(const Scores& sc_) : sc(sc_) {}
-  // which: a bit for each value that is drawn from
-  template <int VEC> __device__ __forceinline__ void operator()(const float (&x)[VEC], int at, unsigned which) {
-    if (!__any_sync(0xffffffffu, which != 0)) return;
-    unsigned may = 0;
+  // of the values no smaller than `lowest`
+  template <int VEC> __device__ __forceinline__ void operator()(const float (&x)[VEC], int at, float lowest) {
+    float big = x[0];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) may |= sc.may_reach(x[i], at + i, enough2) ? 1u << i : 0u;
-    may &= which;
-    for (unsigned left = __reduce_or_sync(0xffffffffu, may); left; left &= left - 1) {
-      const int i = __ffs(left) - 1;
+    for (int i = 1; i < VEC; ++i) big = fmaxf(big, x[i]);
+    if (!__any_sync(0xffffffffu, big >= lowest)) return;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) any |= x[i] >= lowest && sc.may_reach(x[i], at + i, enough2);
+    if (!__any_sync(0xffffffffu, any)) return;
+#pragma unroll 1
+    for (int i = 0; i < VEC; ++i) {
       float y = x[0];
 #pragma unroll
       for (int k = 1; k < VEC; ++k) y = i == k ? x[k] : y;
-      const bool still = (may >> i & 1) && sc.may_reach(y, at + i, enough2);
-      if (!__any_sync(0xffffffffu, still)) continue;
-      if (still) take_better(best.v, best.i, sc.of(y, at + i), at + i);
+      const bool may = y >= lowest && sc.may_reach(y, at + i, enough2);
+      if (!__any_sync(0xffffffffu, may)) continue;
+      if (may) take_better(best.v, best.i, sc.of(y, at + i), at + i);
       const unsigned known = __reduce_max_sync(0xffffffffu, key_of(best.v));
       unsigned of_block = known;
       if ((threadIdx.x & 31) == 0) of_block = max(known, atomicMax(&shared().best_key, known));
@@ -87,28 +90,31 @@ struct Draw {
   }
 };
 
-// The best score of the tokens with c >= cut.
+// The best score of the tokens with c >= cut, which no token of an equal logit is below.
 template <typename T> __device__ __noinline__ Best draw_from(const Scores sc, u64 cut) {
   Draw draw(sc);
   const float lowest = logit_of(cut);
-  const bool ragged = (cut & (MAX_VOCAB - 1)) != 0;    // they begin among equal logits
-  each<T, 2, true>([&](const auto& x, int at) {
-    unsigned which = 0;
-#pragma unroll
-    for (int i = 0; i < 16 / (int)sizeof(T); ++i) which |= x[i] >= lowest ? 1u << i : 0u;
-    if (ragged) {
-#pragma unroll
-      for (int i = 0; i < 16 / (int)sizeof(T); ++i)
-        if (x[i] == lowest && compose(clean(x[i]), at + i) < cut) which &= ~(1u << i);
-    }
-    draw(x, at, which);
-  });
+  each<T, 2, true>([&](const auto& x, int at) { draw(x, at, lowest); });
   return draw.best;
 }
 // Puts the tokens of the range and, with `score`, gives the best score of those above it.
-template <typename T> __device__ __noinline__ Best draw_above(const Scores sc, u64 cut, bool score) {
+template <typename T> __device__ __noinline__ Best draw_above(const Scores sc, bool score) {
+  constexpr int VEC = 16 / (int)sizeof(T);
   Draw draw(sc);
-  put_range<T, true, true>(cut, [&](const auto& x, int at, unsigned which) { if (score) draw(x, at, which); });
+  const u64 high = shared().range.hi;
+  const float next = value_of((unsigned)(high >> INDEX_BITS) + 1);     // the smallest logit above the range's
+  const bool equal = (high & (MAX_VOCAB - 1)) != MAX_VOCAB - 1;        // tokens of the range's largest logit lie above it too
+  put_range<T, true, true>([&](const auto& x, int at) {
+    if (!score) return;
+    if (!equal) {
+      draw(x, at, next);
+      return;
+    }
+    float y[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) y[i] = compose(clean(x[i]), at + i) > high ? x[i] : nan_f();
+    draw(y, at, -INFINITY);
+  });
   return draw.best;
 }
 template <typename T> __device__ __noinline__ Best largest_of_row() {
@@ -281,7 +287,7 @@ __device__ __forceinline__ u64 filtered(const SampleParams& p, const Scores& sc,
       if (!by_mass) return cut;                        // no more tokens than the count leaves
     } else {
       const double above = sh.range.above;
-      best = draw_above<T>(sc, cut, !by_mass);
+      best = draw_above<T>(sc, !by_mass);
       total = send_list();
       const bool last = !by_mass || above == 0.;
       if (!by_mass) {
@@ -306,7 +312,7 @@ __device__ __forceinline__ u64 filtered(const SampleParams& p, const Scores& sc,
     }
   }
   narrow<T, true>(cut, per, LIST / 2, 0., (double)top_p, -1.);
-  best = draw_above<T>(sc, cut, true);
+  best = draw_above<T>(sc, true);
   block_best(best.v, best.i, sh.warp_v, sh.warp_i);
   if (threadIdx.x == 0) { *of(&sh.part_v[sh.rank], 0) = best.v; *of(&sh.part_i[sh.rank], 0) = best.i; }
   total = send_list();

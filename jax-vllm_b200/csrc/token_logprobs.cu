@@ -141,10 +141,11 @@ __global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const ScoreParams
     __syncthreads();
     narrow<T, false>(LOWEST, wide > 0.f ? (float)BINS / wide : 1.f, (unsigned)(LIST - p.top), (double)p.top, -1., -1.);
     // what lies above the range too: fewer than `top`
-    put_range<T, false, false>(LOWEST, [&](const auto& x, int at, unsigned which) {
+    const u64 high = sh.range.hi;
+    put_range<T, false, false>([&](const auto& x, int at) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        if (which >> i & 1) put(compose(clean(x[i]), at + i));
+        if (x[i] == x[i] && compose(clean(x[i]), at + i) > high) put(compose(clean(x[i]), at + i));
     });
     total = send_list();
   }

@@ -74,13 +74,9 @@ template <typename T> __device__ __forceinline__ void unpack(const uint4& raw, f
   }
 }
 
-// A range of tokens that holds the boundary.  While the range is cut into bins of equal width it is given by the distance to
-// the row's largest logit, from <= largest - x < to (as 32 bits round it; no end where `to` is infinite), x no smaller than the
-// lowest logit asked for; once its logits crowd, by lo <= c <= hi.
+// A range of tokens that holds the boundary: lo <= c <= hi.
 struct Range {
   u64 lo, hi;
-  float from, to;
-  bool composed;
   unsigned count;                                      // its tokens (where masses are summed: no fewer than that)
   double above;                                        // tokens, or mass, above it
 };
@@ -483,12 +479,19 @@ static __device__ __noinline__ void sort_list(int m) {
     }
     for (int i = threadIdx.x; i < padded; i += NT) {
       u64 c = sh.list[i];
-      for (int part = size == 32 ? 2 : 32; part <= 32; part *= 2)
-        for (int stride = part / 2; stride > 0; stride /= 2) {
-          const u64 other = __shfl_xor_sync(0xffffffffu, c, stride);
-          const bool down = (i & (size == 32 ? part : size)) == 0, first = (i & stride) == 0;
-          if ((c < other) == (down == first)) c = other;
-        }
+      const auto meet = [&](int stride, bool down) {
+        const u64 other = __shfl_xor_sync(0xffffffffu, c, stride);
+        if ((c < other) == (down == ((i & stride) == 0))) c = other;
+      };
+      if (size == 32) {
+#pragma unroll
+        for (int part = 2; part < 32; part *= 2)
+#pragma unroll
+          for (int stride = part / 2; stride > 0; stride /= 2) meet(stride, (i & part) == 0);
+      }
+      const bool down = (i & size) == 0;
+#pragma unroll
+      for (int stride = 16; stride > 0; stride /= 2) meet(stride, down);
       sh.list[i] = c;
     }
     __syncthreads();
@@ -646,88 +649,94 @@ static __device__ __noinline__ unsigned first_key(unsigned a, unsigned z, float 
 }
 
 // Finds the range of at most `most` tokens, among those with c >= lo, that holds the last token before which the goal is not
-// reached: `goal` tokens, or (MASS) `goal` of the mass, or `part` of the mass of all tokens asked for where part >= 0.  `all` is
-// what all of them make; where that is no more than `plenty`, nothing is looked for.  The first level's bins are 1 / per wide.
+// reached: `goal` tokens, or (MASS) `part` of the mass of all tokens asked for.  `all` is what all of them make; where that is
+// no more than `plenty`, nothing is looked for.  The first level's bins are 1 / per wide.
 template <typename T, bool MASS> __device__ __noinline__ bool narrow(u64 lo, float per, unsigned most, double goal, double part, double plenty) {
   Shared& sh = shared();
   const float largest = sh.largest, deepest = below(logit_of(lo), largest);
-  Range r{lo, compose(largest, 0), 0.f, INFINITY, false, 0u, 0.};
+  // while the range is cut into bins of equal width, it is the tokens with from <= largest - x < to (as 32 bits round it; no end
+  // where `to` is infinite) of those asked for
+  float from = 0.f, to = INFINITY;
+  u64 low = lo, high = compose(largest, 0);
+  bool composed = false;
+  unsigned count = ~0u;
   if (threadIdx.x == 0) sh.range.above = 0.;
-  for (int depth = 0; depth == 0 || r.count > most; ++depth) {
-    if (depth > 0 && !r.composed) {
-      const float wide = fminf(r.to, deepest) - r.from;
+  for (int depth = 0;; ++depth) {
+    if (depth > 0 && !composed) {
+      const float wide = fminf(to, deepest) - from;
       per = (float)BINS / wide;
-      if (depth > 4 || !(wide > 0.f && per > 0.f && per < 1e37f && wide > 1e-6f * fminf(r.to, deepest))) {
-        // logits that crowd, or are equal: from here on by parts of the composed numbers, which end with a single one
-        const unsigned low = (unsigned)(lo >> INDEX_BITS), high = key_of(largest);
-        const u64 bottom = r.to == INFINITY ? lo : (u64)first_key(low, high, r.to) << INDEX_BITS;
-        if (r.from > 0.f) r.hi = ((u64)first_key(low, high, r.from) << INDEX_BITS) - 1;
-        r.lo = bottom > lo ? bottom : lo;
-        r.composed = true;
+      if (count <= most || depth > 4 || !(wide > 0.f && per > 0.f && per < 1e37f && wide > 1e-6f * fminf(to, deepest))) {
+        // it is found, or its logits crowd: from here on a range of composed numbers, of which the parts end with a single one
+        const unsigned a = (unsigned)(lo >> INDEX_BITS), z = key_of(largest);
+        const u64 bottom = to == INFINITY ? lo : (u64)first_key(a, z, to) << INDEX_BITS;
+        if (from > 0.f) high = ((u64)first_key(a, z, from) << INDEX_BITS) - 1;
+        low = bottom > lo ? bottom : lo;
+        composed = true;
       }
     }
+    if (count <= most) break;
     double inside = 0.;
     float least;                                       // the deepest distance that the range may hold
-    if (!r.composed) {
-      const float from = r.from, to = r.to;
+    if (!composed) {
+      const float start = from, end = to;
       per = fminf(per, 1e37f);
-      count_linear<T, MASS>(lo, from, to == INFINITY ? nan_f() : to, per);
+      count_linear<T, MASS>(lo, start, end == INFINITY ? nan_f() : end, per);
       const int b = choose<MASS>(goal, part, depth == 0, inside);
       if (depth == 0 && sh.all <= plenty) return false;
-      const float limit = fminf(to, HUGE_F);
+      const float limit = fminf(end, HUGE_F);
       if (b > 0) {
-        r.from = first_distance(b, from, limit, per);
-        if (r.from >= limit && bin_of(limit, from, per) < b) r.from = INFINITY;          // infinite distances alone
+        from = first_distance(b, start, limit, per);
+        if (from >= limit && bin_of(limit, start, per) < b) from = INFINITY;             // infinite distances alone
       }
       if (b < BINS - 1) {
-        r.to = first_distance(b + 1, from, limit, per);
-        if (r.to >= limit && bin_of(limit, from, per) <= b) r.to = to;
+        to = first_distance(b + 1, start, limit, per);
+        if (to >= limit && bin_of(limit, start, per) <= b) to = end;
       }
-      least = fminf(r.to, deepest);
+      least = fminf(to, deepest);
     } else {
-      const u64 span = r.hi - r.lo, from = r.lo, to = r.hi;
-      const int shift = max(0, 60 - __clzll((long long)span));
-      count_composed<T, MASS>(from, to, shift);
+      const u64 start = low, end = high;
+      const int shift = max(0, 60 - __clzll((long long)(end - start)));
+      count_composed<T, MASS>(start, end, shift);
       const int b = choose<MASS>(goal, part, false, inside);
-      r.lo = from + ((u64)(15 - b) << shift);
-      const u64 end = r.lo + ((1ull << shift) - 1);
-      r.hi = end < to ? end : to;
-      least = below(logit_of(r.lo), largest);
+      low = start + ((u64)(15 - b) << shift);
+      high = low + ((1ull << shift) - 1);
+      if (high > end) high = end;
+      least = below(logit_of(low), largest);
     }
     // no token of the range weighs less than one at its deepest
-    r.count = MASS ? (unsigned)fmin(inside * (double)exp2f(least * sh.scale) * 1.0001 + 1., 4e9) : (unsigned)inside;
+    count = MASS ? (unsigned)fmin(inside * (double)exp2f(least * sh.scale) * 1.0001 + 1., 4e9) : (unsigned)inside;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) { r.above = sh.range.above; sh.range = r; }
+  if (threadIdx.x == 0) {
+    sh.range.lo = low;
+    sh.range.hi = high;
+    sh.range.count = count;
+  }
   __syncthreads();
   return true;
 }
 
-// The tokens of the range, of those with c >= lo, are put; above(values, index of the first, which) is called for the vectors,
-// with a bit for each value that lies above the range, by whole warps where WHOLE.
-template <typename T, bool MASS, bool WHOLE, typename A> __device__ __forceinline__ void put_range(u64 lo, A&& above) {
+// The tokens of the range are put; above(values, index of the first) is called for every vector, by whole warps where WHOLE.
+template <typename T, bool MASS, bool WHOLE, typename A> __device__ __forceinline__ void put_range(A&& above) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  const Range& r = shared().range;
-  const bool composed = r.composed;
-  const float largest = shared().largest, lowest = logit_of(composed ? r.lo : lo), highest = composed ? logit_of(r.hi) : 0.f;
-  const float from = r.from, past = r.to == INFINITY ? nan_f() : r.to;
-  const u64 low = composed ? r.lo : lo, high = r.hi;
+  const u64 low = shared().range.lo, high = shared().range.hi;
+  const float lowest = logit_of(low), highest = logit_of(high);
   const int n = shared().n;
   __syncthreads();                                     // the cells are read: their place is the list's too
   each<T, WHOLE ? 2 : 4, WHOLE>([&](const auto& x, int at) {
-    unsigned which = 0;
+    bool any = false;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float y = asked<MASS>(x[i], at + i, n), d = below(y, largest);
-      bool over = y >= lowest && (composed ? y > highest : d < from);
-      if (y >= lowest && !over && (composed || !(d >= past))) {
-        const u64 c = compose(clean(y), at + i);
-        over = composed && c > high;
-        if (!over && c >= low) put(c);
+    for (int i = 0; i < VEC; ++i) any |= x[i] >= lowest && x[i] <= highest;
+    if (any || lowest == -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float y = asked<MASS>(x[i], at + i, n);
+        if (y >= lowest && y <= highest) {
+          const u64 c = compose(clean(y), at + i);
+          if (c >= low && c <= high) put(c);
+        }
       }
-      which |= over ? 1u << i : 0u;
     }
-    above(x, at, which);
+    above(x, at);
   });
 }
 
