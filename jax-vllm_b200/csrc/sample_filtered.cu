@@ -48,73 +48,108 @@ struct Scores {
   // Whether the score of token i may reach `enough` (given as enough * log2(e)), but for roundings: -log(-log(u)) <= -log(1 - u),
   // and 1 - u is no less than what the first 23 random bits leave of it.
   __device__ __forceinline__ bool may_reach(float x, int i, float enough2) const {
-    const float w = (2.f - 1.1920929e-7f) - __uint_as_float(0x3f800000u | jv_draw_first23(base, (unsigned)i));
+    return bits_may_reach(x, jv_draw_first23(base, (unsigned)i), enough2);
+  }
+  __device__ __forceinline__ bool bits_may_reach(float x, unsigned first23, float enough2) const {
+    const float w = (2.f - 1.1920929e-7f) - __uint_as_float(0x3f800000u | first23);
     return !(w > exp2_fast(fmaf(x, per, -enough2)));
   }
 };
 
-// The best score of the tokens that it is called for, a vector at a time and by whole warps.  What a token can reach at most is
-// compared with the best score that the block knows (which a warp may see late: it only saves work), less what the roundings
-// of both may be (scores are off by a few 2^-24 of themselves, the bound by a few more and by what the approximate exponential
-// lacks): few tokens need their logarithms.
+// The best score of the tokens that it is called for, by whole warps.  What a token can reach at most is compared with the best
+// score that the block knows (which a warp may see late: it only saves work), less what the roundings of both may be (scores
+// are off by a few 2^-24 of themselves, the bound by a few more and by what the approximate exponential lacks): few tokens
+// need their logarithms.
 struct Draw {
   const Scores sc;
   Best best{-INFINITY, 0x7fffffff};
   float enough2 = -INFINITY;
+  int queued = 0;
 
   __device__ __forceinline__ Draw(const Scores& sc_) : sc(sc_) {}
-  // of the values no smaller than `lowest`
-  template <int VEC> __device__ __forceinline__ void operator()(const float (&x)[VEC], int at, float lowest) {
+
+  // One token a lane, NaN: none.
+  __device__ __forceinline__ void one(float y, int i) {
+    const bool may = y == y && sc.may_reach(y, i, enough2);
+    if (!__any_sync(0xffffffffu, may)) return;
+    if (may) take_better(best.v, best.i, sc.of(y, i), i);
+    const unsigned known = __reduce_max_sync(0xffffffffu, key_of(best.v));
+    unsigned of_block = known;
+    if ((threadIdx.x & 31) == 0) of_block = max(known, atomicMax(&shared().best_key, known));
+    const float enough = value_of(__shfl_sync(0xffffffffu, of_block, 0));
+    enough2 = (enough - (1e-5f * fabsf(enough) + 1e-3f)) * LOG2E;
+  }
+  // A vector a lane, every token of it.  The largest logit and the largest random number of the vector bound them all.
+  template <int VEC> __device__ __forceinline__ void all(const float (&x)[VEC], int at) {
     float big = x[0];
+    unsigned luck = 0;
 #pragma unroll
-    for (int i = 1; i < VEC; ++i) big = fmaxf(big, x[i]);
-    if (!__any_sync(0xffffffffu, big >= lowest)) return;
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) any |= x[i] >= lowest && sc.may_reach(x[i], at + i, enough2);
-    if (!__any_sync(0xffffffffu, any)) return;
+    for (int i = 0; i < VEC; ++i) {
+      big = fmaxf(big, x[i]);
+      luck = max(luck, jv_draw_first23(sc.base, (unsigned)(at + i)));
+    }
+    if (!__any_sync(0xffffffffu, sc.bits_may_reach(big, luck, enough2))) return;
 #pragma unroll 1
     for (int i = 0; i < VEC; ++i) {
       float y = x[0];
 #pragma unroll
       for (int k = 1; k < VEC; ++k) y = i == k ? x[k] : y;
-      const bool may = y >= lowest && sc.may_reach(y, at + i, enough2);
-      if (!__any_sync(0xffffffffu, may)) continue;
-      if (may) take_better(best.v, best.i, sc.of(y, at + i), at + i);
-      const unsigned known = __reduce_max_sync(0xffffffffu, key_of(best.v));
-      unsigned of_block = known;
-      if ((threadIdx.x & 31) == 0) of_block = max(known, atomicMax(&shared().best_key, known));
-      const float enough = value_of(__shfl_sync(0xffffffffu, of_block, 0));
-      enough2 = (enough - (1e-5f * fabsf(enough) + 1e-3f)) * LOG2E;
+      one(y, at + i);
     }
+  }
+  // A vector a lane, the tokens of it that are `kept`: they wait until the warp has 32 of them.
+  template <int VEC, typename K> __device__ __forceinline__ void some(const float (&x)[VEC], int at, K&& kept) {
+    uint2* queue = shared().queue[threadIdx.x >> 5];
+    const unsigned before = (1u << (threadIdx.x & 31)) - 1;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const bool is = kept(x[i], at + i);
+      const unsigned who = __ballot_sync(0xffffffffu, is);
+      if (is) queue[queued + __popc(who & before)] = make_uint2(__float_as_uint(x[i]), (unsigned)(at + i));
+      queued += __popc(who);
+    }
+    while (queued >= 32) take(32);
+  }
+  // The last n of the warp's queue.
+  __device__ __forceinline__ void take(int n) {
+    __syncwarp();
+    queued -= n;
+    const int lane = threadIdx.x & 31;
+    const uint2 token = lane < n ? shared().queue[threadIdx.x >> 5][queued + lane] : make_uint2(0x7fffffffu, 0u);
+    __syncwarp();
+    one(__uint_as_float(token.x), (int)token.y);
+  }
+  __device__ __forceinline__ void finish() {
+    if (queued > 0) take(queued);
   }
 };
 
+// The best score of all tokens of the row.
+template <typename T> __device__ __noinline__ Best draw_from_all(const Scores sc) {
+  Draw draw(sc);
+  each<T, 2, true>([&](const auto& x, int at) { draw.all(x, at); });
+  return draw.best;
+}
 // The best score of the tokens with c >= cut, which no token of an equal logit is below.
 template <typename T> __device__ __noinline__ Best draw_from(const Scores sc, u64 cut) {
   Draw draw(sc);
   const float lowest = logit_of(cut);
-  each<T, 2, true>([&](const auto& x, int at) { draw(x, at, lowest); });
+  each<T, 2, true>([&](const auto& x, int at) {
+    draw.some(x, at, [&](float y, int) { return y >= lowest; });
+  });
+  draw.finish();
   return draw.best;
 }
 // Puts the tokens of the range and, with `score`, gives the best score of those above it.
 template <typename T> __device__ __noinline__ Best draw_above(const Scores sc, bool score) {
-  constexpr int VEC = 16 / (int)sizeof(T);
   Draw draw(sc);
   const u64 high = shared().range.hi;
   const float next = value_of((unsigned)(high >> INDEX_BITS) + 1);     // the smallest logit above the range's
   const bool equal = (high & (MAX_VOCAB - 1)) != MAX_VOCAB - 1;        // tokens of the range's largest logit lie above it too
   put_range<T, true, true>([&](const auto& x, int at) {
-    if (!score) return;
-    if (!equal) {
-      draw(x, at, next);
-      return;
-    }
-    float y[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) y[i] = compose(clean(x[i]), at + i) > high ? x[i] : nan_f();
-    draw(y, at, -INFINITY);
+    if (score) draw.some(x, at, [&](float y, int i) { return y >= next || (equal && compose(clean(y), i) > high); });
   });
+  draw.finish();
   return draw.best;
 }
 template <typename T> __device__ __noinline__ Best largest_of_row() {
@@ -347,7 +382,7 @@ __global__ void __launch_bounds__(NT, 2) sample_filtered_kernel(const SamplePara
     started();
   }
   if (cut != 0) {
-    best = hot ? draw_from<T>(sc, cut) : largest_of_row<T>();
+    best = !hot ? largest_of_row<T>() : cut == LOWEST ? draw_from_all<T>(sc) : draw_from<T>(sc, cut);
     block_best(best.v, best.i, sh.warp_v, sh.warp_i);
     if (threadIdx.x == 0) { *of(&sh.part_v[sh.rank], 0) = best.v; *of(&sh.part_i[sh.rank], 0) = best.i; }
     sync_row();
@@ -388,6 +423,6 @@ JV_EXPORT int jv_sample_filtered(const void* logits, int dtype, long long stride
                                  const long long* counters, int* out, int blocks, cudaStream_t stream) {
   if (rows == 0) return JV_OK;
   if (vocab < 1 || vocab > MAX_VOCAB || rows > (1 << 28) || blocks < 0 || blocks > MOST_BLOCKS || (blocks & (blocks - 1))) return JV_ERR_UNSUPPORTED;
-  SampleParams p{logits, stride, rows, vocab, blocks ? blocks : row_blocks(rows, vocab), temperature, top_k, top_p, min_p, seeds, counters, out};
+  SampleParams p{logits, stride, rows, vocab, blocks ? blocks : row_blocks(rows, (long long)vocab * (dtype == 0 ? 4 : 2)), temperature, top_k, top_p, min_p, seeds, counters, out};
   JV_DISPATCH_DTYPE(dtype, T, return launch<T>(p, stream));
 }

@@ -5,6 +5,7 @@
 // A NaN counts as minus infinity; a row that holds nothing else has no likely tokens (every logprob is minus infinity);
 // where the largest logit is infinite, the infinite ones share the probability.
 #include <math.h>
+#include <stddef.h>
 #include "vocab_row.h"
 
 namespace {
@@ -34,7 +35,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 template <typename T> __device__ __noinline__ float2 largest_and_sum() {
   constexpr int VEC = 16 / (int)sizeof(T);
   float m = -INFINITY, s = 0.f;
-  each<T, 8>([&](const auto& x, int) {
+  each<T, 4>([&](const auto& x, int) {
     float big = x[0];
 #pragma unroll
     for (int i = 1; i < VEC; ++i) big = fmaxf(big, x[i]);
@@ -75,8 +76,9 @@ template <typename T> __device__ __noinline__ void list_first(float least) {
   });
 }
 
-template <typename T>
-__global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const ScoreParams p) {
+// Without likely tokens a block needs little memory and few registers: three of them to a multiprocessor.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(NT, TOP ? 2 : 3) token_logprobs_kernel(const ScoreParams p) {
   Shared& sh = shared();
   constexpr int VEC = 16 / (int)sizeof(T);
   pdl_trigger();
@@ -96,11 +98,20 @@ __global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const ScoreParams
     const float v = lane < WARPS ? sh.warp_v[lane] : -INFINITY, block = warp_max(v);
     sum = lane < WARPS ? v == block ? sh.warp_d[0][lane] : sh.warp_d[0][lane] * (double)exp2_fast((v - block) * LOG2E) : 0.;
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane < p.blocks) of(&sh.part[sh.rank][0], lane)[0] = sum;
+    if (lane < p.blocks) {
+      of(&sh.part[sh.rank][0], lane)[0] = sum;
+      if (!TOP) *of(&sh.largest_of[sh.rank], lane) = block;
+    }
   }
-  exchange_largest(mine.x, p.top == 0 ? 1 : (p.top - 1) / p.blocks + 1);
-  if (p.top == 0 && sh.rank != 0 && sh.largest != INFINITY) return;
-  const float largest = sh.largest;
+  float largest = -INFINITY;
+  if (TOP) {
+    exchange_largest(mine.x, (p.top - 1) / p.blocks + 1);
+    largest = sh.largest;
+  } else {
+    sync_row();
+    for (int b = 0; b < p.blocks; ++b) largest = fmaxf(largest, sh.largest_of[b]);
+    if (sh.rank != 0 && largest != INFINITY) return;
+  }
   sum = 0.;
   for (int b = 0; b < p.blocks; ++b) {
     const float v = sh.largest_of[b];
@@ -125,7 +136,7 @@ __global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const ScoreParams
       p.logprob[r] = logprob_of(clean(to_f32(row[token])), largest, log_sum);
     }
   }
-  if (p.top == 0) return;
+  if (!TOP) return;
 
   bool found = false;
   unsigned total = 0;
@@ -158,14 +169,15 @@ __global__ void __launch_bounds__(NT, 2) token_logprobs_kernel(const ScoreParams
   }
 }
 
-template <typename T>
+template <typename T, bool TOP>
 int launch(const ScoreParams& p, cudaStream_t stream) {
+  constexpr int bytes = TOP ? (int)sizeof(Shared) : (int)offsetof(Shared, list);
   static bool done[JV_MAX_DEVICES] = {};
   if (!jv_once_per_device(done, [&] {
-        return cudaFuncSetAttribute(token_logprobs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)) == cudaSuccess;
+        return cudaFuncSetAttribute(token_logprobs_kernel<T, TOP>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
       }))
     return JV_ERR_UNSUPPORTED;
-  return launch_clusters(token_logprobs_kernel<T>, dim3((unsigned)(p.rows * p.blocks)), dim3(NT), sizeof(Shared), p.blocks, stream, p);
+  return launch_clusters(token_logprobs_kernel<T, TOP>, dim3((unsigned)(p.rows * p.blocks)), dim3(NT), bytes, p.blocks, stream, p);
 }
 
 }  // namespace
@@ -177,6 +189,6 @@ JV_EXPORT int jv_token_logprobs(const void* logits, int dtype, long long stride,
   if (rows == 0) return JV_OK;
   if (vocab < 1 || vocab > MAX_VOCAB || rows > (1 << 28) || top < 0 || top > 128 || top > vocab) return JV_ERR_UNSUPPORTED;
   if (blocks < 0 || blocks > MOST_BLOCKS || (blocks & (blocks - 1))) return JV_ERR_UNSUPPORTED;
-  ScoreParams p{logits, stride, rows, vocab, blocks ? blocks : row_blocks(rows, vocab), top, tokens, logprob, top_tokens, top_logprobs, status};
-  JV_DISPATCH_DTYPE(dtype, T, return launch<T>(p, stream));
+  ScoreParams p{logits, stride, rows, vocab, blocks ? blocks : row_blocks(rows, (long long)vocab * (dtype == 0 ? 4 : 2)), top, tokens, logprob, top_tokens, top_logprobs, status};
+  JV_DISPATCH_DTYPE(dtype, T, return top > 0 ? launch<T, true>(p, stream) : launch<T, false>(p, stream));
 }
