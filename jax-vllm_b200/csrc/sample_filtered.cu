@@ -79,7 +79,7 @@ struct Draw {
     const float enough = value_of(__shfl_sync(0xffffffffu, of_block, 0));
     enough2 = (enough - (1e-5f * fabsf(enough) + 1e-3f)) * LOG2E;
   }
-  // A vector a lane, every token of it.  The largest logit and the largest random number of the vector bound them all.
+  // A vector a lane, of every token that is a number.  The largest logit and the largest random number bound them all.
   template <int VEC> __device__ __forceinline__ void all(const float (&x)[VEC], int at) {
     float big = x[0];
     unsigned luck = 0;
@@ -88,7 +88,7 @@ struct Draw {
       big = fmaxf(big, x[i]);
       luck = max(luck, jv_draw_first23(sc.base, (unsigned)(at + i)));
     }
-    if (!__any_sync(0xffffffffu, sc.bits_may_reach(big, luck, enough2))) return;
+    if (!__any_sync(0xffffffffu, big == big && sc.bits_may_reach(big, luck, enough2))) return;
 #pragma unroll 1
     for (int i = 0; i < VEC; ++i) {
       float y = x[0];
@@ -97,16 +97,31 @@ struct Draw {
       one(y, at + i);
     }
   }
-  // A vector a lane, the tokens of it that are `kept`: they wait until the warp has 32 of them.
+  // A vector a lane, of the tokens that are `kept`: where they are few, they wait until the warp has 32 of them.
   template <int VEC, typename K> __device__ __forceinline__ void some(const float (&x)[VEC], int at, K&& kept) {
+    unsigned who[VEC];
+    int number = 0;
+    bool is[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      is[i] = kept(x[i], at + i);
+      who[i] = __ballot_sync(0xffffffffu, is[i]);
+      number += __popc(who[i]);
+    }
+    if (number >= 20 * VEC) {
+      float y[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) y[i] = is[i] ? x[i] : nan_f();
+      all(y, at);
+      return;
+    }
+    if (number == 0) return;
     uint2* queue = shared().queue[threadIdx.x >> 5];
     const unsigned before = (1u << (threadIdx.x & 31)) - 1;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const bool is = kept(x[i], at + i);
-      const unsigned who = __ballot_sync(0xffffffffu, is);
-      if (is) queue[queued + __popc(who & before)] = make_uint2(__float_as_uint(x[i]), (unsigned)(at + i));
-      queued += __popc(who);
+      if (is[i]) queue[queued + __popc(who[i] & before)] = make_uint2(__float_as_uint(x[i]), (unsigned)(at + i));
+      queued += __popc(who[i]);
     }
     while (queued >= 32) take(32);
   }
@@ -354,7 +369,7 @@ __device__ __forceinline__ u64 filtered(const SampleParams& p, const Scores& sc,
   drawn = true;
   if (sh.rank != 0) return ~0ull;
   sort_list((int)total);
-  listed = kept_by_mass((int)total, sh.range.above, (double)top_p, sh.all, list_mass);
+  listed = kept_by_mass((int)total, sh.range.above, (double)top_p, sh.range.all, list_mass);
   return 0;
 }
 

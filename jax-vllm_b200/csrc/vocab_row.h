@@ -74,11 +74,14 @@ template <typename T> __device__ __forceinline__ void unpack(const uint4& raw, f
   }
 }
 
-// A range of tokens that holds the boundary: lo <= c <= hi.
+// A range of tokens that holds the boundary: lo <= c <= hi.  While it is cut into bins of equal width, it is the tokens with
+// from <= largest - x < to (as 32 bits round it; no end where `to` is infinite) of those asked for.
 struct Range {
   u64 lo, hi;
-  unsigned count;                                      // its tokens (where masses are summed: no fewer than that)
-  double above;                                        // tokens, or mass, above it
+  float from, to, per;                                 // bins 1 / per wide
+  int shift;                                           // bins of 2^shift composed numbers
+  bool composed, found, enough;                        // enough: as few tokens as were looked for, or fewer, are all there are
+  double above, all;                                   // tokens, or mass, above it and of all that were asked for
 };
 
 struct Shared {
@@ -98,7 +101,6 @@ struct Shared {
   float largest, scale, bound;                         // bound: at least `j * blocks` tokens are no smaller; scale: log2(e) / T
   Range range;
   u64 told;                                            // the boundary, from the first block
-  double all;                                          // tokens, or mass, of all that were asked for
   unsigned listed, mine, base, best_key;
   // (a kernel that lists and counts nothing has no memory from here on)
   alignas(16) u64 list[LIST];
@@ -599,10 +601,9 @@ template <typename T, bool MASS> __device__ __noinline__ void count_composed(u64
   });
 }
 
-// After every block has counted: the bin of the boundary, the last one that has tokens and before which `goal` (tokens, or
-// `part` of the whole mass where part >= 0) is not reached.  Takes range.above and range.count over to that bin's (the count
-// only where tokens are counted; else the bin's mass is returned in `inside`); `first`: `all` gets the sum of all bins.
-template <bool MASS> __device__ __noinline__ int choose(double goal, double part, bool first, double& inside) {
+// After every block has counted: the sums of the bins over the blocks' threads go to every block.  Holds one barrier of the
+// cluster.
+template <bool MASS> __device__ __noinline__ void add_bins() {
   Shared& sh = shared();
   __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = sh.blocks, parity = sh.parity;
@@ -625,31 +626,6 @@ template <bool MASS> __device__ __noinline__ int choose(double goal, double part
     if (lane < blocks) *of(&sh.bins[parity][sh.rank][b], lane) = q;
   }
   sync_row();
-  // what lies above a lane's bin is what the lanes before it have
-  double q = 0;
-  if (lane < BINS)
-    for (int k = 0; k < blocks; ++k) q += sh.bins[parity][k][lane];
-  double to = q;
-  for (int o = 1; o < 32; o *= 2) {
-    const double other = __shfl_up_sync(0xffffffffu, to, o);
-    if (lane >= o) to += other;
-  }
-  const double all = first ? __shfl_sync(0xffffffffu, to, 31) : sh.all;
-  double above = __shfl_up_sync(0xffffffffu, to, 1);
-  above = sh.range.above + (lane == 0 ? 0. : above);
-  const double end = part >= 0. ? part * all : goal;
-  const unsigned holds = __ballot_sync(0xffffffffu, lane < BINS && q > 0. && (above == 0. || above < end));
-  const int l = holds ? 31 - __clz(holds) : 0;
-  above = __shfl_sync(0xffffffffu, above, l);
-  inside = __shfl_sync(0xffffffffu, q, l);
-  __syncthreads();                                     // the last level's sums are read
-  if (threadIdx.x == 0) {
-    sh.range.above = above;
-    sh.parity = parity ^ 1;
-    if (first) sh.all = all;
-  }
-  __syncthreads();
-  return l;
 }
 
 // The smallest distance in bin b or deeper, of those from `from` to `to` (which is given where there is none).
@@ -690,71 +666,93 @@ static __device__ __noinline__ unsigned first_key(unsigned a, unsigned z, float 
   return z;
 }
 
+// The first warp, after a level: takes the range over to the bin of the boundary, the last one that has tokens and before which
+// the goal is not reached.
+template <bool MASS> __device__ __noinline__ void take_bin(u64 lo, unsigned most, double goal, double part, double plenty, int depth) {
+  Shared& sh = shared();
+  Range& r = sh.range;
+  const int lane = threadIdx.x & 31;
+  const float largest = sh.largest, deepest = below(logit_of(lo), largest);
+  // what lies above a lane's bin is what the lanes before it have
+  double q = 0;
+  if (lane < BINS)
+    for (int k = 0; k < sh.blocks; ++k) q += sh.bins[sh.parity][k][lane];
+  double sum = q;
+  for (int o = 1; o < 32; o *= 2) {
+    const double other = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += other;
+  }
+  const double all = depth == 0 ? __shfl_sync(0xffffffffu, sum, 31) : r.all;
+  double above = __shfl_up_sync(0xffffffffu, sum, 1);
+  above = r.above + (lane == 0 ? 0. : above);
+  const double end = part >= 0. ? part * all : goal;
+  const unsigned holds = __ballot_sync(0xffffffffu, lane < BINS && q > 0. && (above == 0. || above < end));
+  const int b = holds ? 31 - __clz(holds) : 0;
+  above = __shfl_sync(0xffffffffu, above, b);
+  const double inside = __shfl_sync(0xffffffffu, q, b);
+  const bool enough = depth == 0 && all <= plenty;
+
+  float from = r.from, to = r.to, per = r.per, least;  // least: the deepest distance that the range may hold
+  u64 low = r.lo, high = r.hi;
+  bool composed = r.composed;
+  if (!composed) {
+    const float limit = fminf(to, HUGE_F);
+    float first = from, last = to;
+    if (b > 0) {
+      first = first_distance(b, from, limit, per);
+      if (first >= limit && bin_of(limit, from, per) < b) first = INFINITY;            // infinite distances alone
+    }
+    if (b < BINS - 1) {
+      last = first_distance(b + 1, from, limit, per);
+      if (last >= limit && bin_of(limit, from, per) <= b) last = to;
+    }
+    from = first;
+    to = last;
+    least = fminf(to, deepest);
+  } else {
+    low += (u64)(15 - b) << r.shift;
+    const u64 last = low + ((1ull << r.shift) - 1);
+    if (last < high) high = last;
+    least = below(logit_of(low), largest);
+  }
+  // its tokens (where masses are summed, no fewer than that: no token of the range weighs less than one at its deepest)
+  const unsigned count = MASS ? (unsigned)fmin(inside * (double)exp2f(least * sh.scale) * 1.0001 + 1., 4e9) : (unsigned)inside;
+  const bool found = count <= most;
+  if (!composed && !enough) {
+    const float wide = fminf(to, deepest) - from;
+    per = (float)BINS / wide;
+    if (found || depth > 3 || !(wide > 0.f && per > 0.f && per < 1e37f && wide > 1e-6f * fminf(to, deepest))) {
+      // the logits crowd, or it is found: a range of composed numbers, of which the parts end with a single one
+      const unsigned a = (unsigned)(lo >> INDEX_BITS), z = key_of(largest);
+      const u64 bottom = to == INFINITY ? lo : (u64)first_key(a, z, to) << INDEX_BITS;
+      if (from > 0.f) high = ((u64)first_key(a, z, from) << INDEX_BITS) - 1;
+      low = bottom > lo ? bottom : lo;
+      composed = true;
+    }
+  }
+  __syncwarp();
+  if (lane == 0)
+    r = Range{low, high, from, to, fminf(per, 1e37f), max(0, 60 - __clzll((long long)(high - low))), composed, found, enough, above, all};
+  if (lane == 0) sh.parity ^= 1;
+}
+
 // Finds the range of at most `most` tokens, among those with c >= lo, that holds the last token before which the goal is not
-// reached: `goal` tokens, or (MASS) `part` of the mass of all tokens asked for.  `all` is what all of them make; where that is
-// no more than `plenty`, nothing is looked for.  The first level's bins are 1 / per wide.
+// reached: `goal` tokens, or (MASS) `part` of the mass of all tokens asked for.  range.all is what all of them make; where
+// that is no more than `plenty`, nothing is looked for.  The first level's bins are 1 / per wide.
 template <typename T, bool MASS> __device__ __noinline__ bool narrow(u64 lo, float per, unsigned most, double goal, double part, double plenty) {
   Shared& sh = shared();
-  const float largest = sh.largest, deepest = below(logit_of(lo), largest);
-  // while the range is cut into bins of equal width, it is the tokens with from <= largest - x < to (as 32 bits round it; no end
-  // where `to` is infinite) of those asked for
-  float from = 0.f, to = INFINITY;
-  u64 low = lo, high = compose(largest, 0);
-  bool composed = false;
-  unsigned count = ~0u;
-  if (threadIdx.x == 0) sh.range.above = 0.;
-  for (int depth = 0;; ++depth) {
-    if (depth > 0 && !composed) {
-      const float wide = fminf(to, deepest) - from;
-      per = (float)BINS / wide;
-      if (count <= most || depth > 4 || !(wide > 0.f && per > 0.f && per < 1e37f && wide > 1e-6f * fminf(to, deepest))) {
-        // it is found, or its logits crowd: from here on a range of composed numbers, of which the parts end with a single one
-        const unsigned a = (unsigned)(lo >> INDEX_BITS), z = key_of(largest);
-        const u64 bottom = to == INFINITY ? lo : (u64)first_key(a, z, to) << INDEX_BITS;
-        if (from > 0.f) high = ((u64)first_key(a, z, from) << INDEX_BITS) - 1;
-        low = bottom > lo ? bottom : lo;
-        composed = true;
-      }
-    }
-    if (count <= most) break;
-    double inside = 0.;
-    float least;                                       // the deepest distance that the range may hold
-    if (!composed) {
-      const float start = from, end = to;
-      per = fminf(per, 1e37f);
-      count_linear<T, MASS>(lo, start, end == INFINITY ? nan_f() : end, per);
-      const int b = choose<MASS>(goal, part, depth == 0, inside);
-      if (depth == 0 && sh.all <= plenty) return false;
-      const float limit = fminf(end, HUGE_F);
-      if (b > 0) {
-        from = first_distance(b, start, limit, per);
-        if (from >= limit && bin_of(limit, start, per) < b) from = INFINITY;             // infinite distances alone
-      }
-      if (b < BINS - 1) {
-        to = first_distance(b + 1, start, limit, per);
-        if (to >= limit && bin_of(limit, start, per) <= b) to = end;
-      }
-      least = fminf(to, deepest);
-    } else {
-      const u64 start = low, end = high;
-      const int shift = max(0, 60 - __clzll((long long)(end - start)));
-      count_composed<T, MASS>(start, end, shift);
-      const int b = choose<MASS>(goal, part, false, inside);
-      low = start + ((u64)(15 - b) << shift);
-      high = low + ((1ull << shift) - 1);
-      if (high > end) high = end;
-      least = below(logit_of(low), largest);
-    }
-    // no token of the range weighs less than one at its deepest
-    count = MASS ? (unsigned)fmin(inside * (double)exp2f(least * sh.scale) * 1.0001 + 1., 4e9) : (unsigned)inside;
-  }
-  if (threadIdx.x == 0) {
-    sh.range.lo = low;
-    sh.range.hi = high;
-    sh.range.count = count;
-  }
   __syncthreads();
-  return true;
+  if (threadIdx.x == 0) sh.range = Range{lo, compose(sh.largest, 0), 0.f, INFINITY, fminf(per, 1e37f), 0, false, false, false, 0., 0.};
+  __syncthreads();
+  for (int depth = 0;; ++depth) {
+    if (sh.range.composed) count_composed<T, MASS>(sh.range.lo, sh.range.hi, sh.range.shift);
+    else count_linear<T, MASS>(lo, sh.range.from, sh.range.to == INFINITY ? nan_f() : sh.range.to, sh.range.per);
+    add_bins<MASS>();
+    if (threadIdx.x < 32) take_bin<MASS>(lo, most, goal, part, plenty, depth);
+    __syncthreads();
+    if (sh.range.enough) return false;
+    if (sh.range.found) return true;
+  }
 }
 
 // The tokens of the range are put; above(values, index of the first) is called for every vector, by whole warps where WHOLE.
