@@ -383,7 +383,7 @@ static __device__ __noinline__ unsigned send_list() {
 // infinity is not put, nor what lies more than `deepest` below the largest.  Returns this thread's largest logit and, SUMMED,
 // the sum of its masses, relative to that one's.
 template <typename T, bool SUMMED> __device__ __noinline__ float2 put_once(int j, float deepest) {
-  constexpr int VEC = 16 / (int)sizeof(T), AHEAD = 4;
+  constexpr int VEC = 16 / (int)sizeof(T), AHEAD = 6;
   const float scale = shared().scale;
   const int vectors = shared().vectors;
   float m = -INFINITY, s = 0.f, least = INFINITY;
@@ -408,17 +408,12 @@ template <typename T, bool SUMMED> __device__ __noinline__ float2 put_once(int j
   };
   const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(shared().row) + shared().head) + threadIdx.x;
   int at = shared().head + threadIdx.x * VEC;
-  uint4 next[AHEAD];                                   // the loads of the round to come are on their way during one
-#pragma unroll
-  for (int u = 0; u < AHEAD; ++u) next[u] = (int)threadIdx.x + u * NT < vectors ? p[u * NT] : no_vector();
   for (int k = 0; k == 0 || k * AHEAD * NT < vectors; ++k) {
     uint4 raw[AHEAD];
+    const int left = vectors - k * AHEAD * NT - (int)threadIdx.x;
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) raw[u] = next[u];
+    for (int u = 0; u < AHEAD; ++u) raw[u] = left > u * NT ? p[u * NT] : no_vector();
     p += AHEAD * NT;
-    const int left = vectors - (k + 1) * AHEAD * NT - (int)threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) next[u] = left > u * NT ? p[u * NT] : no_vector();
     if (k == 0 || k == 3) {                            // what the first vectors hold above their own bound
       float g = m;
       if (k == 0) {
