@@ -86,6 +86,7 @@ int copy_some(const Plane* planes, int n_planes, const Pairs& pairs, int first, 
   return jv_launch(page_copy_kernel<V, PLANES, PAIRS>, dim3((unsigned)(wanted < most ? wanted : most)), dim3(THREADS), 0, stream, job);
 }
 
+// Parameters of a launch are copied with it: as few as serve (0.8 KB to 18 KB).
 constexpr int FEW_PLANES = 4, FEW_PAIRS = 32, MANY_PLANES = 64, MANY_PAIRS = 1024;
 
 template <typename V>
@@ -93,8 +94,11 @@ int copy_all(const Plane* planes, int n_planes, const Pairs& pairs, cudaStream_t
   for (int p = 0; p < n_planes; p += MANY_PLANES)
     for (int i = 0; i < pairs.n; i += MANY_PAIRS) {
       const int np = n_planes - p < MANY_PLANES ? n_planes - p : MANY_PLANES, ni = pairs.n - i < MANY_PAIRS ? pairs.n - i : MANY_PAIRS;
-      const int rc = np <= FEW_PLANES && ni <= FEW_PAIRS ? copy_some<V, FEW_PLANES, FEW_PAIRS>(planes + p, np, pairs, i, ni, stream)
-                                                         : copy_some<V, MANY_PLANES, MANY_PAIRS>(planes + p, np, pairs, i, ni, stream);
+      const bool few_planes = np <= FEW_PLANES, few_pairs = ni <= FEW_PAIRS;
+      const int rc = few_planes && few_pairs ? copy_some<V, FEW_PLANES, FEW_PAIRS>(planes + p, np, pairs, i, ni, stream)
+                     : few_planes            ? copy_some<V, FEW_PLANES, MANY_PAIRS>(planes + p, np, pairs, i, ni, stream)
+                     : few_pairs             ? copy_some<V, MANY_PLANES, FEW_PAIRS>(planes + p, np, pairs, i, ni, stream)
+                                             : copy_some<V, MANY_PLANES, MANY_PAIRS>(planes + p, np, pairs, i, ni, stream);
       if (rc != JV_OK) return rc;
     }
   return JV_OK;

@@ -12,6 +12,7 @@ another size while requests live.
 
 from __future__ import annotations
 
+import contextlib
 import threading
 import time
 import weakref
@@ -144,6 +145,19 @@ def add_continuations(driver: Driver, prompt_ids, n: int, sampling=None) -> list
     return [req.request_id for req in reqs]
 
 
+@contextlib.contextmanager
+def _device_idle(driver: Driver):
+    """What is done to the cache between two steps, on whatever stream the caller has, begins after the steps issued so far
+    and is done before the next one."""
+    device = torch.device(driver.config.device)
+    if device.type != "cuda":
+        yield
+        return
+    torch.cuda.synchronize(device)
+    yield
+    torch.cuda.synchronize(device)
+
+
 def fork_request(driver: Driver, request_id: int, sampling: Optional[SamplingParams] = None) -> int:
     """Adds a request that goes on from where an unfinished one stands; returns its id.  It shares the full pages that the
     other holds and takes a copy of the last page and of the states; without a free slot or page it waits and is computed
@@ -163,7 +177,8 @@ def fork_request(driver: Driver, request_id: int, sampling: Optional[SamplingPar
         child = _new_request(driver, parent.prompt_ids, sp)
         child.output_ids = list(parent.output_ids)
         driver.requests[child.request_id] = child
-        driver.scheduler.fork(parent, [child])
+        with _device_idle(driver):
+            driver.scheduler.fork(parent, [child])
     driver.router.wake()
     return child.request_id
 
@@ -189,7 +204,8 @@ def resize_cache(driver: Driver, num_blocks: int) -> None:
         driver.ahead = None
         if hasattr(driver.runner, "forget_graphs"):
             driver.runner.forget_graphs()
-        cache.resize(num_blocks)
+        with _device_idle(driver):
+            cache.resize(num_blocks)
         if torch.device(driver.config.device).type == "cuda":
             torch.cuda.empty_cache()             # what the old stores held goes back to the device
         sched.version += 1

@@ -2744,15 +2744,14 @@ def copy_slots(states, src, dst) -> None:
     pairs = check_copies("copy_slots", src, dst, slots, slots, False)
     planes, device = [], None
     for t in states:
-        if not isinstance(t, torch.Tensor) or t.dim() < 1 or t.shape[0] != slots:
+        if not isinstance(t, torch.Tensor) or t.dim() < 1 or t.size(0) != slots:
             raise KernelError("copy_slots: all states are [slots, ...] with the same number of slots")
-        if device is None or t.get_device() != device:
+        if t.get_device() != device:
             device = t.get_device()
             _on_current_device("copy_slots", device)
-        at, size = t.data_ptr(), t.nbytes
-        if not size:
+        at, row = t.data_ptr(), t.nbytes // slots if slots else 0
+        if not row:
             continue
-        row = size // slots
         step = row
         if not t.is_contiguous():
             step = t.stride(0) * t.element_size()
