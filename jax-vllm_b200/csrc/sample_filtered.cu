@@ -10,6 +10,15 @@
 // vocab_row.h, and only they need a random number.  Tokens with (largest - x) / T > 30 are left out from the start where
 // there is a filter: their mass is below 1e-13 of the largest's, and -log(-log(u)) lies between -2.9 and 16.7 (but for the
 // one u in 2^24 that rounds to 1), so that they cannot be drawn before the largest.
+//
+// What bounds it, and what it takes (alone on the device, calls behind one another): one row of 151,936 logits 10.4 us, a chain of
+// two passes over 76 KB a block (2.4 and 1.8 us) and two barriers of the cluster with what they carry (2.3 and 1.5 us); 256 rows of which
+// the first 40 tokens are kept 36.6 us, the memory's 23.8 and the ends of the rows' chains, which nothing covers; 64 nearly even
+// rows under top-p 77 us, instructions: 5 a logit for the largest, 17 for each of two levels, 46 for the random number of a kept one.
+// Tried and dropped: one pass with a bound from the row's start for clusters too (as a block by itself does it: 18 -> 31
+// instructions a logit), the next round's loads ahead of a round (copies between registers: 46 -> 58 a drawn logit), and for
+// top-p a draw from all tokens, repeated among those before it while it is not kept (138 -> 109 a logit, but a step waits for the
+// row with the most rounds: 77 -> 100 us).
 #include "sampling.h"
 #include "vocab_row.h"
 
@@ -202,48 +211,53 @@ template <typename T, bool SUMMED> __device__ __noinline__ float2 list_first(flo
   return make_float2(all, listed);
 }
 
-// First block only: the mass of the list's first m tokens, and how many of them have less than `part` of the mass that counts
-// before them (with `above` before the first): `mass`, or the list's where that is negative.
+// First block only: how many of the list's first m tokens have less than `part` of the mass that counts before them, with `above`
+// before the first: `mass`, or the list's where that is negative.  `sum`: the list's.  A list of no more than 128 tokens is
+// one warp's work.
 static __device__ __noinline__ int kept_by_mass(int m, double above, double part, double mass, double& sum) {
   constexpr int PER = LIST / NT;
   Shared& sh = shared();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float largest = sh.largest, scale = sh.scale;
-  double q[PER], s = 0.;
+  const int warps = m <= 32 * PER ? 1 : WARPS;
+  double to = 0., q[PER], s = 0.;
+  if (warp < warps) {
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int i = PER * threadIdx.x + j;
-    q[j] = i < m ? (double)exp2_fast(-(below(logit_of(sh.list[i]), largest) * scale)) : 0.;
-    s += q[j];
+    for (int j = 0; j < PER; ++j) {
+      const int i = PER * threadIdx.x + j;
+      q[j] = i < m ? (double)exp2_fast(-(below(logit_of(sh.list[i]), largest) * scale)) : 0.;
+      s += q[j];
+    }
+    to = s;
+    for (int o = 1; o < 32; o *= 2) {
+      const double t = __shfl_up_sync(0xffffffffu, to, o);
+      if (lane >= o) to += t;
+    }
+    if (lane == 31) sh.warp_d[0][warp] = to;
   }
-  double to = s;
-  for (int o = 1; o < 32; o *= 2) {
-    const double t = __shfl_up_sync(0xffffffffu, to, o);
-    if (lane >= o) to += t;
-  }
-  __syncthreads();
-  if (lane == 31) sh.warp_d[0][warp] = to;
   __syncthreads();
   double before = above, total = 0.;
-  for (int w = 0; w < WARPS; ++w) {
+  for (int w = 0; w < warps; ++w) {
     if (w < warp) before += sh.warp_d[0][w];
     total += sh.warp_d[0][w];
   }
   sum = total;
-  const double first = __shfl_up_sync(0xffffffffu, to, 1), end = part * (mass < 0. ? total : mass);
-  if (lane > 0) before += first;
-  int mine = 0;
+  if (warp < warps) {
+    const double first = __shfl_up_sync(0xffffffffu, to, 1), end = part * (mass < 0. ? total : mass);
+    if (lane > 0) before += first;
+    int mine = 0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int i = PER * threadIdx.x + j;
-    if (i < m && (before == 0. || before < end)) mine = i + 1;
-    before += q[j];
+    for (int j = 0; j < PER; ++j) {
+      const int i = PER * threadIdx.x + j;
+      if (i < m && (before == 0. || before < end)) mine = i + 1;
+      before += q[j];
+    }
+    mine = __reduce_max_sync(0xffffffffu, mine);
+    if (lane == 0) sh.warp_i[warp] = mine;
   }
-  mine = __reduce_max_sync(0xffffffffu, mine);
-  if (lane == 0) sh.warp_i[warp] = mine;
   __syncthreads();
   int kept = 0;
-  for (int w = 0; w < WARPS; ++w) kept = max(kept, sh.warp_i[w]);
+  for (int w = 0; w < warps; ++w) kept = max(kept, sh.warp_i[w]);
   __syncthreads();
   return kept;
 }
@@ -379,11 +393,11 @@ __global__ void __launch_bounds__(NT, 2) sample_filtered_kernel(const SamplePara
   pdl_trigger();
   pdl_wait();
   const int r = blockIdx.x / p.blocks;
-  begin(reinterpret_cast<const T*>(p.logits) + (size_t)r * p.stride, p.vocab, p.blocks);
   const float temp = p.temperature[r];
   const int top_k = p.top_k[r];
   const float top_p = p.top_p[r], min_p = p.min_p[r];
   const Scores sc{temp, LOG2E / temp, jv_draw_base((u64)p.seeds[r], (u64)p.counters[r])};
+  begin(reinterpret_cast<const T*>(p.logits) + (size_t)r * p.stride, p.vocab, p.blocks);
   if (sh.rank == 0 && threadIdx.x == 0) p.out[r] = 0;
   Best best{-INFINITY, 0x7fffffff};
   int listed = 0;                                      // first block: kept tokens of its sorted list
@@ -406,11 +420,18 @@ __global__ void __launch_bounds__(NT, 2) sample_filtered_kernel(const SamplePara
   }
   if (listed > 0) {
     best = Best{-INFINITY, 0x7fffffff};
-    for (int i = threadIdx.x; i < listed; i += NT) {
+    const int threads = listed <= 64 ? 32 : NT;        // few tokens are one warp's work
+    if ((int)threadIdx.x >= threads) return;
+    for (int i = threadIdx.x; i < listed; i += threads) {
       const u64 c = sh.list[i];
       take_better(best.v, best.i, sc.of(logit_of(c), index_of(c)), index_of(c));
     }
-    block_best(best.v, best.i, sh.warp_v, sh.warp_i);
+    if (threads == 32) {
+      for (int o = 16; o > 0; o >>= 1)
+        take_better(best.v, best.i, __shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.i, o));
+    } else {
+      block_best(best.v, best.i, sh.warp_v, sh.warp_i);
+    }
   }
   if (threadIdx.x == 0) {
     if (drawn)

@@ -6,7 +6,7 @@
 // A token weighs exp((x - largest) / T) in 32 bits; sums are 32-bit within a thread, 64-bit across threads, in a fixed order.
 //
 // Few first tokens are found in two passes.  In the first every thread keeps its largest logit.  The j-th largest of a block's
-// (of 128 groups of four threads, or of the threads where j is large) has at least j tokens at or above it in that block, and
+// (of its warps, of 128 groups of four threads, or of the threads where j is large) has at least j tokens at or above it in that block, and
 // not many more in a row whose large logits lie anywhere; the lowest of the blocks' bounds therefore has at least j * blocks
 // in the row.  The second pass puts the tokens at or above the bound in a list, which the first block sorts.
 //
@@ -277,40 +277,63 @@ __device__ __forceinline__ bool countable(int j, int blocks) {
 // where a block has too few threads with any).  Holds one barrier of the cluster.
 static __device__ __noinline__ void exchange_largest(float m, int j) {
   Shared& sh = shared();
-  float g = m;
+  const int blocks = sh.blocks;
+  if (j <= WARPS / 2) {
+    // the warps' own largest do, and the first warp finds the place of each
+    const unsigned k = __reduce_max_sync(0xffffffffu, key_of(m + 0.f));
+    if (threadIdx.x % 32 == 0) sh.warp_i[threadIdx.x / 32] = (int)k;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const unsigned mine = threadIdx.x < WARPS ? (unsigned)sh.warp_i[threadIdx.x] : 0u;
+      int above = 0, reach = 0;
 #pragma unroll
-  for (int o = 1; o < GROUP; o *= 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-  const int part = threadIdx.x % GROUP, blocks = sh.blocks;
-  if (part == 0) sh.group[threadIdx.x / GROUP] = g;
-  __syncthreads();
-  // the groups above this one's largest, and those at it: each of its lanes compares with a share of the others
-  int both = 0;
-  const float4* others = reinterpret_cast<const float4*>(sh.group);
-#pragma unroll 4
-  for (int i = 0; i < GROUPS / 4 / GROUP; ++i) {
-    const float4 o = others[i * GROUP + part];
-    both += ((o.x > g) + (o.y > g) + (o.z > g) + (o.w > g)) << 16;
-    both += (o.x >= g) + (o.y >= g) + (o.z >= g) + (o.w >= g);
-  }
-#pragma unroll
-  for (int o = 1; o < GROUP; o *= 2) both += __shfl_xor_sync(0xffffffffu, both, o);
-  const int above = both >> 16, reach = both & 0xffff;
-  if (above == 0)                                      // (equal ones write the same)
-    for (int b = part; b < blocks; b += GROUP) *of(&sh.largest_of[sh.rank], b) = g;
-  if (j <= FEW) {
-    if (above < j && reach >= j)
-      for (int b = part; b < blocks; b += GROUP) *of(&sh.bound_of[sh.rank], b) = g;
-  } else {
-    // the threads' own largest: a key that j of them reach, by halves
-    unsigned lo = KEY_LOWEST, hi = 0xff800000u;        // at least j reach lo; fewer reach beyond hi
-    const unsigned mine = key_of(m + 0.f);
-    while (lo < hi) {
-      const unsigned mid = lo + (hi - lo) / 2 + 1;
-      const int c = __syncthreads_count(mine >= mid);
-      if (c >= j) lo = mid; else hi = mid - 1;
-      if (c >= j && c <= j + j / 16) break;
+      for (int w = 0; w < WARPS; ++w) {
+        const unsigned o = __shfl_sync(0xffffffffu, mine, w);
+        above += o > mine;
+        reach += o >= mine;
+      }
+      if (threadIdx.x < WARPS)
+        for (int b = 0; b < blocks; ++b) {             // (equal ones write the same)
+          if (above == 0) *of(&sh.largest_of[sh.rank], b) = value_of(mine);
+          if (above < j && reach >= j) *of(&sh.bound_of[sh.rank], b) = value_of(mine);
+        }
     }
-    if (threadIdx.x < blocks) *of(&sh.bound_of[sh.rank], threadIdx.x) = value_of(lo);
+  } else {
+    float g = m;
+#pragma unroll
+    for (int o = 1; o < GROUP; o *= 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    const int part = threadIdx.x % GROUP;
+    if (part == 0) sh.group[threadIdx.x / GROUP] = g;
+    __syncthreads();
+    // the groups above this one's largest, and those at it: each of its lanes compares with a share of the others
+    int both = 0;
+    const float4* others = reinterpret_cast<const float4*>(sh.group);
+#pragma unroll 4
+    for (int i = 0; i < GROUPS / 4 / GROUP; ++i) {
+      const float4 o = others[i * GROUP + part];
+      both += ((o.x > g) + (o.y > g) + (o.z > g) + (o.w > g)) << 16;
+      both += (o.x >= g) + (o.y >= g) + (o.z >= g) + (o.w >= g);
+    }
+#pragma unroll
+    for (int o = 1; o < GROUP; o *= 2) both += __shfl_xor_sync(0xffffffffu, both, o);
+    const int above = both >> 16, reach = both & 0xffff;
+    if (above == 0)                                    // (equal ones write the same)
+      for (int b = part; b < blocks; b += GROUP) *of(&sh.largest_of[sh.rank], b) = g;
+    if (j <= FEW) {
+      if (above < j && reach >= j)
+        for (int b = part; b < blocks; b += GROUP) *of(&sh.bound_of[sh.rank], b) = g;
+    } else {
+      // the threads' own largest: a key that j of them reach, by halves
+      unsigned lo = KEY_LOWEST, hi = 0xff800000u;      // at least j reach lo; fewer reach beyond hi
+      const unsigned mine = key_of(m + 0.f);
+      while (lo < hi) {
+        const unsigned mid = lo + (hi - lo) / 2 + 1;
+        const int c = __syncthreads_count(mine >= mid);
+        if (c >= j) lo = mid; else hi = mid - 1;
+        if (c >= j && c <= j + j / 16) break;
+      }
+      if (threadIdx.x < blocks) *of(&sh.bound_of[sh.rank], threadIdx.x) = value_of(lo);
+    }
   }
   sync_row();
   // (every warp for itself; they write the same)
