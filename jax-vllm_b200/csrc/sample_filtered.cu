@@ -196,8 +196,10 @@ template <typename T, bool SUMMED> __device__ __noinline__ float2 list_first(flo
 #pragma unroll
     for (int i = 1; i < VEC; ++i) big = fmaxf(big, x[i]);
     if (SUMMED) {
+      float q[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) all += x[i] >= low ? exp2_fast(-(below(x[i], largest) * scale)) : 0.f;
+      for (int i = 0; i < VEC; ++i) q[i] = x[i] >= low ? exp2_fast(-(below(x[i], largest) * scale)) : 0.f;
+      all += sum_of(q);
     }
     if (big >= least) {
 #pragma unroll
@@ -276,7 +278,7 @@ __device__ __forceinline__ u64 filtered(const SampleParams& p, const Scores& sc,
   const bool can_list = countable(j, p.blocks);
   const bool summed = by_mass && !by_count;            // the mass that counts is that of the whole row
   // one block a row: one pass, unless the mass that counts depends on the largest logit
-  const bool once = p.blocks == 1 && (by_count || by_mass) && can_list && !(summed && by_share);
+  const bool once = p.blocks == 1 && (by_count || by_mass) && can_list && fits_once<T>(j, p.vocab) && !(summed && by_share);
   if (threadIdx.x == 0) sh.scale = fminf(fmaxf(sc.per, 1e-37f), 3e38f);
   float2 mine{-INFINITY, 0.f};
   if (once) {

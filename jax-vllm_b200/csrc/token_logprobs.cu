@@ -45,8 +45,10 @@ template <typename T, int AHEAD> __device__ __noinline__ float2 largest_and_sum(
       s *= exp2_fast((m - big) * LOG2E);
       m = big;
     }
+    float q[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) s += exp2_fast(fmaxf(x[i] - m, -1000.f) * LOG2E);
+    for (int i = 0; i < VEC; ++i) q[i] = exp2_fast(fmaxf(x[i] - m, -1000.f) * LOG2E);
+    s += sum_of(q);
   });
   return make_float2(m, s);
 }

@@ -74,6 +74,18 @@ template <typename T> __device__ __forceinline__ void unpack(const uint4& raw, f
   }
 }
 
+// By pairs: a thread adds a vector's sum to its own, which is rounded once for every vector.
+template <int VEC> __device__ __forceinline__ float sum_of(const float (&x)[VEC]) {
+  float s[VEC / 2];
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) s[i] = x[2 * i] + x[2 * i + 1];
+#pragma unroll
+  for (int n = VEC / 4; n > 0; n /= 2)
+#pragma unroll
+    for (int i = 0; i < n; ++i) s[i] += s[i + n];
+  return s[0];
+}
+
 // A range of tokens that holds the boundary: lo <= c <= hi.  While it is cut into bins of equal width, it is the tokens with
 // from <= largest - x < to (as 32 bits round it; no end where `to` is infinite) of those asked for.
 struct Range {
@@ -401,6 +413,13 @@ static __device__ __noinline__ unsigned send_list() {
   return total;
 }
 
+// Whether what put_once puts is likely to have room: what the first vectors hold above their bound, and as much again whenever as
+// many have been read as the bound was taken of.
+template <typename T> __device__ __forceinline__ bool fits_once(int j, int n) {
+  const float first = 6.f * NT * (16 / sizeof(T)), all = (float)n;
+  const float own = (float)NT * -__logf(1.f - (float)j * (1.f / NT));
+  return own * (1.f + fmaxf(0.f, fminf(all, 3.f * first) - first) / first + fmaxf(0.f, all - 3.f * first) / (3.f * first)) < 0.75f * LIST;
+}
 // One pass instead of two, where one block reads a row: the bound for j tokens of what has been read so far, taken after the
 // first vectors and once more later, decides what is put, so that the list gets more tokens than it has to hold.  Minus
 // infinity is not put, nor what lies more than `deepest` below the largest.  Returns this thread's largest logit and, SUMMED,
@@ -419,8 +438,10 @@ template <typename T, bool SUMMED> __device__ __noinline__ float2 put_once(int j
     if (SUMMED) {
       if (big > m) s *= exp2_fast(-(fminf(big - m, HUGE_F) * scale));
       const float to = fmaxf(big, m);
+      float q[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s += x[i] > -INFINITY ? exp2_fast(-(below(x[i], to) * scale)) : 0.f;
+      for (int i = 0; i < VEC; ++i) q[i] = x[i] > -INFINITY ? exp2_fast(-(below(x[i], to) * scale)) : 0.f;
+      s += sum_of(q);
     }
     m = fmaxf(m, big);
     if (big >= least) {

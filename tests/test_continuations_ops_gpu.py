@@ -38,9 +38,11 @@ def test_uniforms_of_this_file_are_the_package_s():
 
 
 # A mass exp((x - largest) / T) is formed in 32 bits: the difference, log2(e) / T and their product are each off by half a step
-# (2^-24), which in the exponent makes 3 * 2^-24 * d for d = (largest - x) / T, and exp2f adds two steps (2^-22).  A mass with
-# d > 30 is below 2^-43 of the largest and counts as nothing.  So sums are off by less than 90 * 2^-24 + 2^-22 = 5.7e-6 of
-# themselves, plus 2^-43 of the largest mass for each token that was cut.
+# (2^-24), which in the exponent makes 3 * 2^-24 * d for d = (largest - x) / T, and the exponential adds two steps (2^-22).
+# Tokens with d > 30 are below 2^-43 of the largest mass and may be left out.  Weighed by the masses themselves, d is no more than
+# log(151936) = 12 on the average, so the masses put sums off by 40 * 2^-24 = 2.4e-6 of themselves.  A thread adds up to 75 vectors'
+# sums, half a step each (75 * 2^-24 = 4.5e-6 where one block reads a row), across threads in 64 bits.  Both sides of a border
+# are such sums: 2 * (2.4e-6 + 4.5e-6) = 1.4e-5; twice 5.7e-6 is asked for.
 def accepted(x, t, k, p, m, seed, counter):
     """The tokens that a row may give: exact but where a border, or two scores, lie nearer than 32 bits tell apart."""
     x = np.where(np.isnan(x), -INF, x) + 0.0
