@@ -146,6 +146,7 @@ class CacheManager:
         self.prefix_cache = bool(prefix_cache) and not self.state_layers
         self.live: dict[object, RequestCache] = {}
         self.views: dict = {}                # what allocate_storage handed out, by (layer or (layer, member))
+        self.broken: Optional[str] = None    # why the stores and the tables no longer agree (a resize that ended half done)
         self.stats = {"prefix_hit_pages": 0, "prefix_hit_tokens": 0, "pages_allocated": 0, "pages_released": 0,
                       "pages_shared": 0, "pages_copied": 0}
 
@@ -340,10 +341,36 @@ class CacheManager:
     def resize(self, num_pages: int) -> None:
         """Gives every group `num_pages` pages: what live requests hold, and as many of the pages kept for reuse as fit, move
         to the first pages of new stores; the views that `allocate_storage` handed out follow.  One store at a time: the
-        old and the new one exist beside each other while their pages are copied."""
+        old and the new one exist beside each other while their pages are copied.  What cannot be done is refused before
+        anything has changed; should an allocation fail all the same, the cache is `broken` and takes no more steps."""
         if num_pages < 1:
             raise ValueError("a pool needs at least one page")
-        pools = [grp.pool.resized(num_pages) for grp in self.groups]      # raises before anything has changed
+        self._check_room(num_pages)
+        pools = [grp.pool.resized(num_pages) for grp in self.groups]
+        try:
+            self._move(num_pages, pools)
+        except BaseException as exc:
+            self.broken = f"the pool of pages was left half resized by {type(exc).__name__}: {exc}"
+            raise
+
+    def _stores(self) -> list:
+        return [t for grp in self.groups for t in ((grp.k,) if grp.v is grp.k else (grp.k, grp.v)) if t is not None]
+
+    def _check_room(self, num_pages: int) -> None:
+        """Refuses new stores that would not fit beside the old ones that are left when each is allocated."""
+        extra = most = 0
+        for old in self._stores():
+            new = old.nbytes // old.shape[1] * num_pages
+            most = max(most, extra + new)
+            extra += new - old.nbytes
+        device = next((t.device for t in self._stores()), None)
+        if device is not None and device.type == "cuda":
+            torch.cuda.empty_cache()             # what no tensor holds goes back to the device, so that it counts as free
+            free = torch.cuda.mem_get_info(device)[0]
+            if most > free:
+                raise ValueError(f"{num_pages} pages need {most} bytes of device memory while they take over the old ones, {free} are free")
+
+    def _move(self, num_pages: int, pools: list) -> None:
         for g, (grp, (pool, moved)) in enumerate(zip(self.groups, pools)):
             for name in ("k",) if grp.v is grp.k else ("k", "v"):
                 old = getattr(grp, name)

@@ -23,6 +23,7 @@ import torch
 
 from ..cache import CacheManager
 from ..config import EngineConfig, parse_dtype
+from ..ops import MOST_VOCAB
 from ..sampling import Sampler
 from .background import EventRouter
 from .batch import StepEntry
@@ -97,6 +98,13 @@ def _checked_prompt(driver: Driver, prompt_ids) -> list:
     return prompt
 
 
+def _check_sampling(driver: Driver, prompt: list, sampling: SamplingParams) -> None:
+    driver.scheduler.validate(prompt, sampling)
+    vocab = driver.model.spec.vocab_size
+    if vocab > MOST_VOCAB and (sampling.filtered or sampling.logprobs is not None):
+        raise ValueError(f"filters and log-probabilities are for at most {MOST_VOCAB} tokens, the vocabulary has {vocab}")
+
+
 def _new_request(driver: Driver, prompt: list, sampling: SamplingParams) -> Request:
     with driver.id_lock:
         rid = driver.next_id
@@ -109,7 +117,7 @@ def add_request(driver: Driver, prompt_ids, sampling: Optional[SamplingParams] =
     driver.router.raise_if_failed()
     sp = sampling or SamplingParams()
     prompt = _checked_prompt(driver, prompt_ids)
-    driver.scheduler.validate(prompt, sp)
+    _check_sampling(driver, prompt, sp)
     req = _new_request(driver, prompt, sp)
     with driver.step_lock:
         driver.requests[req.request_id] = req
@@ -134,7 +142,7 @@ def add_continuations(driver: Driver, prompt_ids, n: int, sampling=None) -> list
         raise ValueError("one set of sampling parameters for all continuations, or one for each")
     prompt = _checked_prompt(driver, prompt_ids)
     for sp in sampling:
-        driver.scheduler.validate(prompt, sp)
+        _check_sampling(driver, prompt, sp)
     reqs = [_new_request(driver, prompt, sp) for sp in sampling]
     reqs[0].followers = reqs[1:]
     with driver.step_lock:
@@ -168,12 +176,12 @@ def fork_request(driver: Driver, request_id: int, sampling: Optional[SamplingPar
         parent = driver.requests.get(request_id)
         if parent is None or parent.finished:
             raise KeyError(f"request {request_id} is not running")
-        if any(parent in r.followers for r in driver.requests.values()):
+        if any(parent is f for r in list(driver.requests.values()) for f in r.followers):
             raise ValueError(f"request {request_id} waits for the prompt that it continues")
         sp = sampling if sampling is not None else replace(parent.sampling, seed=None)
         if len(parent.output_ids) >= sp.max_new_tokens:
             raise ValueError(f"the request has {len(parent.output_ids)} tokens already, max_new_tokens is {sp.max_new_tokens}")
-        driver.scheduler.validate(parent.prompt_ids, sp)
+        _check_sampling(driver, parent.prompt_ids, sp)
         child = _new_request(driver, parent.prompt_ids, sp)
         child.output_ids = list(parent.output_ids)
         driver.requests[child.request_id] = child
@@ -226,6 +234,8 @@ def step(driver: Driver) -> list:
 
 def _step_locked(driver: Driver) -> list:
     sched = driver.scheduler
+    if driver.cache.broken:
+        raise RuntimeError(driver.cache.broken)
     ahead, driver.ahead = driver.ahead, None
     plan = sched.take_ahead(ahead) or sched.schedule()
     if not plan:
@@ -262,19 +272,28 @@ def _step_locked(driver: Driver) -> list:
     if not sampled:
         return events
     if both is None:
-        if forking:
-            rows = [row for row, _ in draws]
-            logits = driver.sampler.repeat_rows(logits, rows) if logits.is_cuda else logits[rows]
-        if filters is None:
-            tokens = driver.sampler.sample(logits, temps, seeds, counters)
-        else:
-            tokens = driver.sampler.sample_filtered(logits, temps, seeds, counters, filters)
-        parts = [tokens, driver.runner.status_word()]
+        parts = [[], [], [], []]
+        # a prompt's continuations need its row once each: of hundreds, no more rows at a time than requests run at a time
+        at_once = max(len(sampled), driver.max_num_seqs, 64) if forking else len(draws)
+        for i in range(0, len(draws), at_once):
+            part = slice(i, i + at_once)
+            block = logits
+            if forking:
+                rows = [row for row, _ in draws[part]]
+                block = driver.sampler.repeat_rows(logits, rows) if logits.is_cuda else logits[rows]
+            if filters is None:
+                tokens = driver.sampler.sample(block, temps[part], seeds[part], counters[part])
+            else:
+                tokens = driver.sampler.sample_filtered(block, temps[part], seeds[part], counters[part], filters[part])
+            parts[0].append(tokens)
+            if top >= 0:
+                chosen, top_tokens, top_values = driver.sampler.logprobs(block, tokens, top)
+                parts[1].append(chosen.view(torch.int32))
+                parts[2].append(top_tokens.reshape(-1))
+                parts[3].append(top_values.view(torch.int32).reshape(-1))
         if top >= 0:
-            chosen, top_tokens, top_values = driver.sampler.logprobs(logits, tokens, top)
             top = top_tokens.shape[1]
-            parts += [chosen.view(torch.int32), top_tokens.reshape(-1), top_values.view(torch.int32).reshape(-1)]
-        both = torch.cat(parts)                                          # one copy back
+        both = torch.cat([*parts[0], driver.runner.status_word(), *parts[1], *parts[2], *parts[3]])      # one copy back
     arrived = None
     if both.is_cuda:
         # the copy is on its way while the host plans the next step; waiting for it also synchronises

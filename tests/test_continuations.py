@@ -266,3 +266,47 @@ def test_the_pool_changes_its_size_between_steps():
         d.cache.check()
     assert [q.output_ids for q in reqs] == [expected(p, 12, i) for i, p in enumerate(prompts)]
     assert generate(d, prompts, SamplingParams(max_new_tokens=3, seed=1)) == [expected(p, 3, 1) for p in prompts]
+
+
+def test_more_continuations_than_rows_at_a_time():
+    d, r = driver(max_num_seqs=3, max_model_len=64, block_size=4)
+    rows = []
+    sample = d.sampler.sample
+    d.sampler.sample = lambda logits, *a: rows.append(logits.shape[0]) or sample(logits, *a)
+    reqs = continuations(d, [4, 5, 6], 150, SamplingParams(max_new_tokens=2, seed=0))
+    assert [q.output_ids for q in reqs] == [expected([4, 5, 6], 2, i) for i in range(150)]
+    assert rows[:3] == [64, 64, 22] and max(rows[3:]) <= 3
+    d.cache.check()
+
+
+def test_filters_and_scores_of_a_vocabulary_that_is_too_large_are_refused(monkeypatch):
+    d, _ = driver(max_num_seqs=2, max_model_len=32, block_size=4)
+    from jax_vllm_b200.engine import engine
+    monkeypatch.setattr(engine, "MOST_VOCAB", VOCAB - 1)
+    for sp in (SamplingParams(max_new_tokens=2, temperature=1.0, top_k=3), SamplingParams(max_new_tokens=2, logprobs=0)):
+        with pytest.raises(ValueError):
+            add_request(d, [1], sp)
+        with pytest.raises(ValueError):
+            add_continuations(d, [1], 2, sp)
+        i = add_request(d, [1], SamplingParams(max_new_tokens=4, seed=0))
+        with pytest.raises(ValueError):
+            fork_request(d, i, sp)
+    assert generate(d, [[1]], SamplingParams(max_new_tokens=2, temperature=1.0, seed=0)) == [expected([1], 2, 0)]
+
+
+def test_a_pool_that_was_left_half_resized_takes_no_more_steps(monkeypatch):
+    d, _ = driver(max_num_seqs=2, max_model_len=32, block_size=4, num_blocks=12)
+    i = add_request(d, [1, 2, 3, 4, 5], SamplingParams(max_new_tokens=9, seed=0))
+    step(d)
+    with pytest.raises(ValueError):
+        resize_cache(d, 1)
+    assert d.cache.broken is None and step(d)
+
+    def no_memory(*a):
+        raise torch.OutOfMemoryError("no memory")
+    monkeypatch.setattr(d.cache, "_move", no_memory)
+    with pytest.raises(torch.OutOfMemoryError):
+        resize_cache(d, 9)
+    with pytest.raises(RuntimeError, match="half resized"):
+        step(d)
+    assert not d.requests[i].finished

@@ -177,6 +177,10 @@ def test_a_pool_of_another_size_between_steps(setup):
             d.cache.check()
     assert [r.output_ids for r in reqs] == want
     resize_cache(d, 64)
+    page = sum(t.nbytes for g in d.cache.groups for t in (g.k, g.v)) // 64
+    with pytest.raises(ValueError, match="device memory"):
+        resize_cache(d, (1 << 39) // page)             # three times what the device has
+    assert d.cache.num_pages == 64
     assert generate(d, prompts, SamplingParams(max_new_tokens=20)) == want    # prefixes that moved along among them
     assert d.stats.cache_hit_tokens > 0
 
