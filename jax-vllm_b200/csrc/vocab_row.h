@@ -693,6 +693,13 @@ static __device__ __noinline__ float first_distance(int b, float from, float to,
 static __device__ __noinline__ unsigned first_key(unsigned a, unsigned z, float to) {
   const int lane = threadIdx.x & 31;
   const float largest = shared().largest;
+  // it lies within a step of where it would without rounding
+  const float guess = largest - to, some = fmaxf(to, fabsf(largest)) * 2.4e-7f;
+  const unsigned early = key_of(guess - some), late = key_of(guess + some);
+  if (early >= a && late <= z && early < late && !(below(value_of(early), largest) < to) && below(value_of(late), largest) < to) {
+    a = early + 1;
+    z = late;
+  }
   while (a < z) {
     const unsigned step = (z - a + 31) / 32, p = min(z - 1, a + lane * step);
     const unsigned yes = __ballot_sync(0xffffffffu, below(value_of(p), largest) < to);
