@@ -349,7 +349,7 @@ __device__ __forceinline__ u64 filtered(const SampleParams& p, const Scores& sc,
   const float step = DEEPEST * temp, wide = 6.f * (largest - sh.bound);
   const float per = (float)BINS / (wide > 0.f ? fminf(step, wide) : step);
   if (by_count) {                                      // the boundary by count
-    if (!narrow<T, false>(cut, per, LIST / 2, (double)top_k, -1., (double)top_k)) {
+    if (!narrow<T, false>(cut, per, LIST, (double)top_k, -1., (double)top_k)) {
       if (!by_mass) return cut;                        // no more tokens than the count leaves
     } else {
       const double above = sh.range.above;
@@ -377,7 +377,7 @@ __device__ __forceinline__ u64 filtered(const SampleParams& p, const Scores& sc,
       sync_row();                                      // it is read: the first block may go on to another one
     }
   }
-  narrow<T, true>(cut, per, LIST / 2, 0., (double)top_p, -1.);
+  narrow<T, true>(cut, per, LIST, 0., (double)top_p, -1.);
   best = draw_above<T>(sc, true);
   block_best(best.v, best.i, sh.warp_v, sh.warp_i);
   if (threadIdx.x == 0) { *of(&sh.part_v[sh.rank], 0) = best.v; *of(&sh.part_i[sh.rank], 0) = best.i; }
