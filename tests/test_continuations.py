@@ -1,13 +1,16 @@
 """Continuations of one prompt, forks and pools that change their size, with a stand-in for the device (no GPU): what the
 cache manager and the scheduler decide, and what the entry point refuses."""
 
+import random
+import threading
+
 import pytest
 import torch
 
 from jax_vllm_b200 import registry
 from jax_vllm_b200.cache import CacheManager, OutOfPages, PagePool
 from jax_vllm_b200.engine import (SamplingParams, add_continuations, add_request, continuations, fork_request, generate, has_work, make_driver,
-                                  resize_cache, step)
+                                  resize_cache, start, step, stop, stream)
 from jax_vllm_b200.parts import BuildContext, FixedStateNeed, Model, PagedKVNeed
 from tests.test_scheduler import FakeRunner, next_token
 from tests.util import TINY_A
@@ -310,3 +313,41 @@ def test_a_pool_that_was_left_half_resized_takes_no_more_steps(monkeypatch):
     with pytest.raises(RuntimeError, match="half resized"):
         step(d)
     assert not d.requests[i].finished
+
+
+def test_continuations_forks_and_sizes_from_several_threads():
+    d, _ = driver(max_num_seqs=5, max_model_len=64, block_size=4, max_tokens_per_step=16, num_blocks=60)
+    faults = []
+
+    def work(k):
+        r = random.Random(k)
+        try:
+            for _ in range(6):
+                prompt = [r.randrange(VOCAB) for _ in range(r.randrange(1, 30))]
+                ids = add_continuations(d, prompt, r.randrange(1, 6), SamplingParams(max_new_tokens=12, seed=k))
+                for _ in range(2):
+                    try:
+                        f = fork_request(d, ids[0], SamplingParams(max_new_tokens=20, seed=k))
+                        got = [e.token for e in stream(d, f)]
+                        assert got == expected(prompt, 20, k)[20 - len(got):]
+                    except KeyError:                   # it has finished
+                        pass
+                    try:
+                        resize_cache(d, r.randrange(20, 80))
+                    except ValueError:                 # too few pages for what is live
+                        pass
+                for i, rid in enumerate(ids):
+                    assert [e.token for e in stream(d, rid)] == expected(prompt, 12, k + i)
+        except BaseException as exc:
+            faults.append(exc)
+
+    start(d)
+    threads = [threading.Thread(target=work, args=(k,), daemon=True) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not faults and not any(t.is_alive() for t in threads) and d.router.failure is None
+    stop(d)
+    d.cache.check()
+    assert not d.cache.live and not d.requests

@@ -215,3 +215,31 @@ def test_continuations_and_forks_of_every_kind_of_cache(family, tag, tmp_path):
     assert [r.output_ids for r in reqs] == [want[0], want[0]]
     d.cache.check()
     assert not d.cache.live
+
+
+@pytest.mark.parametrize("family,tag", [("nufapel", "na"), ("gogivik", "ga"), ("nasedra", "na"), ("guronex", "ga"), ("tidarax", None), ("loselix", None)])
+def test_more_continuations_than_slots_and_pages(family, tag, tmp_path):
+    """Some are forked, some wait, some are preempted and computed again; a request is forked in the middle of its prompt."""
+    from jax_vllm_b200 import SamplingParams, add_continuations, add_request, fork_request, generate, has_work, load_from_path, make_driver, step
+    util = importlib.import_module(f"tests.{family}_util")
+    tag = tag or sorted(util.CONFIGS)[0]
+    c = util.CONFIGS[tag]
+    folder = util.write_folder(tmp_path / "m", c, util.make_weights(c, 5))
+    model = load_from_path(folder, dtype="fp32")
+    vocab, P = model.spec.vocab_size, util.PAGE[tag]
+    prompt, other = random_tokens(2 * P + 3, vocab, seed=17), random_tokens(3 * P + 1, vocab, seed=18)
+    sp = [SamplingParams(max_new_tokens=P + 6, temperature=0.9, top_p=0.95, seed=170 + i) for i in range(7)]
+    alone = make_driver(model, max_num_seqs=1, max_model_len=6 * P, block_size=P)
+    want = [generate(alone, [prompt], s)[0] for s in sp]
+    want_other = generate(alone, [other], sp[0])[0]
+    d = make_driver(model, max_num_seqs=4, max_model_len=6 * P, block_size=P, num_blocks=11, max_tokens_per_step=2 * P)
+    a = add_request(d, other, sp[0])
+    step(d)                                            # a part of its prompt
+    b = fork_request(d, a, sp[0])
+    ids = add_continuations(d, prompt, 7, sp)
+    reqs = [d.requests[i] for i in [a, b] + ids]
+    while has_work(d):
+        step(d)
+        d.cache.check()
+    assert [r.output_ids for r in reqs] == [want_other, want_other] + want
+    assert d.stats.forks > 1 and not d.cache.live
