@@ -243,3 +243,37 @@ def test_more_continuations_than_slots_and_pages(family, tag, tmp_path):
         d.cache.check()
     assert [r.output_ids for r in reqs] == [want_other, want_other] + want
     assert d.stats.forks > 1 and not d.cache.live
+
+
+def test_command_line_and_class(tmp_path):
+    """cli.py and LLM as a user calls them: the continuations, their tokens and log-probabilities are the entry point's."""
+    import json, os, subprocess, sys
+    from pathlib import Path
+    from jax_vllm_b200 import LLM, SamplingParams
+    folder = make_folder(tmp_path / "m", "a", seed=6)
+    root = Path(__file__).resolve().parent.parent
+    prompts = [random_tokens(n, TINY["a"]["vocab_size"], seed=1300 + n) for n in (9, 21)]
+    cmd = [sys.executable, str(root / "cli.py"), "--model-path", str(folder), "--dtype", "fp32", "--max-tokens", "6", "--max-model-len", "64",
+           "--block-size", str(PAGE_SIZE["a"]), "--temperature", "0.7", "--top-k", "30", "--top-p", "0.9", "--min-p", "0.01", "--seed", "5",
+           "--n", "3", "--logprobs", "2"]
+    for p in prompts:
+        cmd += ["--prompt-ids", ",".join(map(str, p))]
+    out = subprocess.run(cmd, capture_output=True, text=True, timeout=600, cwd=str(root), env=dict(os.environ))
+    assert out.returncode == 0, out.stderr[-2000:]
+    got = [json.loads(line) for line in out.stdout.splitlines() if line.startswith("{")]
+    llm = LLM(folder, dtype="fp32", max_num_seqs=4, max_model_len=64, block_size=PAGE_SIZE["a"])
+    want = [r for i, p in enumerate(prompts)
+            for r in llm.continuations(p, 3, SamplingParams(max_new_tokens=6, temperature=0.7, top_k=30, top_p=0.9, min_p=0.01, seed=5 + 3 * i, logprobs=2))]
+    assert [g["output_ids"] for g in got] == [r.output_ids for r in want]
+    for g, r in zip(got, want):
+        assert len(g["logprobs"]) == 6 and [[t for t, _ in step] for step in g["top_logprobs"]] == [[t for t, _ in step] for step in r.top_logprobs]
+        # log-probabilities of logits that lie within LOGITS of the plain ones differ by twice that at most, those of two runs by four times
+        assert max(abs(a - b) for a, b in zip(g["logprobs"], r.logprobs)) <= 4 * LOGITS
+    i = llm.add_request(prompts[0], SamplingParams(max_new_tokens=8))
+    llm.step()
+    j = llm.fork_request(i)
+    llm.resize_cache(llm.driver.num_blocks + 1)
+    first, second = llm.driver.requests[i], llm.driver.requests[j]
+    while llm.has_work():
+        llm.step()
+    assert first.output_ids == second.output_ids and len(first.output_ids) == 8
