@@ -8,8 +8,8 @@
 //   T == 0       the largest logit
 // Every filter leaves the first tokens up to a boundary, so the kept ones are a range of the composed numbers of
 // vocab_row.h, and only they need a random number.  Tokens with (largest - x) / T > 30 are left out from the start where
-// there is a filter: their mass is below 1e-13 of the largest's, and -log(-log(u)) lies between -2.9 and 16.7 (but for the
-// one u in 2^24 that rounds to 1), so that they cannot be drawn before the largest.
+// there is a filter: their mass is below 1e-13 of the largest's, and -log(-log(u)) lies between -2.9 and 16.7, so that they
+// cannot be drawn before the largest.
 //
 // What bounds it, and what it takes (alone on the device, calls behind one another): one row of 151,936 logits 10.4 us, a chain of
 // two passes over 76 KB a block (2.4 and 1.8 us) and two barriers of the cluster with what they carry (2.3 and 1.5 us); 256 rows of which
@@ -52,7 +52,7 @@ struct Scores {
   u64 base;
 
   __device__ __forceinline__ float of(float x, int i) const {
-    return x / temp - logf(-logf(((float)(unsigned)(jv_draw_bits(base, (unsigned)i) >> 40) + 0.5f) * (1.0f / 16777216.0f)));
+    return x / temp - logf(-logf(jv_uniform_of(jv_draw_bits(base, (unsigned)i))));
   }
   // Whether the score of token i may reach `enough` (given as enough * log2(e)), but for roundings: -log(-log(u)) <= -log(1 - u),
   // and 1 - u is no less than what the first 23 random bits leave of it.

@@ -10,8 +10,7 @@ __host__ __device__ __forceinline__ unsigned long long jv_mix64(unsigned long lo
   return z ^ (z >> 31);
 }
 
-// What the numbers of one (seed, counter) have in common, and the 64 random bits of its vocabulary index v: jv_uniform is
-// ((bits >> 40) + 0.5) / 2^24 in 32 bits.
+// What the numbers of one (seed, counter) have in common, and the 64 random bits of its vocabulary index v.
 __host__ __device__ __forceinline__ unsigned long long jv_draw_base(unsigned long long seed, unsigned long long counter) {
   return jv_mix64(seed + 0x9E3779B97F4A7C15ULL * (counter + 1));
 }
@@ -27,11 +26,14 @@ __host__ __device__ __forceinline__ unsigned jv_draw_first23(unsigned long long 
   return (unsigned)(z >> 41);
 }
 
-// Uniform in (0, 1) with 24 random bits.
+// Uniform in (0, 1) with 24 of them: (n + 1/2) / 2^24, rounded to 32 bits.  The topmost would round to 1, whose score
+// -log(-log(u)) is infinite: it is the largest number below.
+__host__ __device__ __forceinline__ float jv_uniform_of(unsigned long long bits) {
+  return fminf(((float)(unsigned)(bits >> 40) + 0.5f) * (1.0f / 16777216.0f), 1.0f - 1.0f / 16777216.0f);
+}
 __host__ __device__ __forceinline__ float jv_uniform(unsigned long long seed, unsigned long long counter,
                                                      unsigned long long v) {
-  const unsigned long long h = jv_draw_bits(jv_draw_base(seed, counter), v);
-  return ((float)(unsigned)(h >> 40) + 0.5f) * (1.0f / 16777216.0f);
+  return jv_uniform_of(jv_draw_bits(jv_draw_base(seed, counter), v));
 }
 
 // (value, index) ordering: larger value wins, the lower index among equal values.

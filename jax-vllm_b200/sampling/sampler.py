@@ -26,7 +26,8 @@ def mix64(z: int) -> int:
 
 def uniform(seed: int, counter: int, v: int) -> float:
     """The uniform number in (0, 1) that the kernel uses for vocabulary index v (a host
-    restatement, for tests and for reasoning about reproducibility)."""
+    restatement, for tests and for reasoning about reproducibility).  The kernel rounds it to
+    32 bits: it is at most 2^-25 off there, and never 1."""
     h = mix64((seed + 0x9E3779B97F4A7C15 * (counter + 1)) & _MASK64)
     h = mix64(h ^ ((v * 0xD1342543DE82EF95 + 0x2545F4914F6CDD1D) & _MASK64))
     return ((h >> 40) + 0.5) / 16777216.0
