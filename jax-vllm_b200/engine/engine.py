@@ -105,25 +105,36 @@ def _check_sampling(driver: Driver, prompt: list, sampling: SamplingParams) -> N
         raise ValueError(f"filters and log-probabilities are for at most {MOST_VOCAB} tokens, the vocabulary has {vocab}")
 
 
-def _new_request(driver: Driver, prompt: list, sampling: SamplingParams) -> Request:
+def _new_request(driver: Driver, prompt: list, sampling: SamplingParams, arrival: Optional[float] = None) -> Request:
     with driver.id_lock:
         rid = driver.next_id
         driver.next_id += 1
     driver.router.open(rid)
-    return Request(request_id=rid, prompt_ids=prompt, sampling=sampling, arrival=time.perf_counter())
+    return Request(request_id=rid, prompt_ids=prompt, sampling=sampling, arrival=time.perf_counter() if arrival is None else arrival)
+
+
+def _add(driver: Driver, prompt: list, sampling: list) -> list:
+    """Registers requests that continue one prompt, the first of them with the scheduler; returns their ids."""
+    arrival = time.perf_counter()
+    for sp in sampling:
+        _check_sampling(driver, prompt, sp)      # what is refused anyway need not wait for a step
+    with driver.step_lock:
+        # the pool may have changed its size meanwhile: all are checked before anything of them is registered
+        for sp in sampling:
+            _check_sampling(driver, prompt, sp)
+        reqs = [_new_request(driver, prompt, sp, arrival) for sp in sampling]
+        reqs[0].followers = reqs[1:]
+        for req in reqs:
+            driver.requests[req.request_id] = req
+        driver.scheduler.add(reqs[0])
+    driver.router.wake()
+    return [req.request_id for req in reqs]
 
 
 def add_request(driver: Driver, prompt_ids, sampling: Optional[SamplingParams] = None) -> int:
     driver.router.raise_if_failed()
     sp = sampling or SamplingParams()
-    prompt = _checked_prompt(driver, prompt_ids)
-    _check_sampling(driver, prompt, sp)
-    req = _new_request(driver, prompt, sp)
-    with driver.step_lock:
-        driver.requests[req.request_id] = req
-        driver.scheduler.add(req)
-    driver.router.wake()
-    return req.request_id
+    return _add(driver, _checked_prompt(driver, prompt_ids), [sp])[0]
 
 
 def add_continuations(driver: Driver, prompt_ids, n: int, sampling=None) -> list:
@@ -140,17 +151,7 @@ def add_continuations(driver: Driver, prompt_ids, n: int, sampling=None) -> list
         sampling = [replace(one, seed=None if one.seed is None else one.seed + i) for i in range(n)]
     if len(sampling) != n:
         raise ValueError("one set of sampling parameters for all continuations, or one for each")
-    prompt = _checked_prompt(driver, prompt_ids)
-    for sp in sampling:
-        _check_sampling(driver, prompt, sp)
-    reqs = [_new_request(driver, prompt, sp) for sp in sampling]
-    reqs[0].followers = reqs[1:]
-    with driver.step_lock:
-        for req in reqs:
-            driver.requests[req.request_id] = req
-        driver.scheduler.add(reqs[0])
-    driver.router.wake()
-    return [req.request_id for req in reqs]
+    return _add(driver, _checked_prompt(driver, prompt_ids), sampling)
 
 
 @contextlib.contextmanager

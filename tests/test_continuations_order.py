@@ -1,0 +1,82 @@
+"""Continuations, forks and sizes that meet one another, with a stand-in for the device (no GPU)."""
+
+import threading
+
+import pytest
+
+from jax_vllm_b200.engine import SamplingParams, add_continuations, add_request, has_work, resize_cache, step
+from jax_vllm_b200.engine import engine as eng
+from tests.test_continuations import driver, expected
+
+
+def resized_on_the_way(monkeypatch, d, num_blocks):
+    """Another thread asks for a pool of another size at the moment at which the engine makes its next request record.
+    Returns the function that ends that thread, and what it was refused with, if it was."""
+    refused, made = [], eng._new_request
+
+    def other():
+        try:
+            resize_cache(d, num_blocks)
+        except ValueError as exc:
+            refused.append(exc)
+    thread = threading.Thread(target=other, daemon=True)
+
+    def new_request(*a, **k):
+        if not thread.is_alive() and thread.ident is None:
+            thread.start()
+            thread.join(0.5)                           # it may have to wait for this request
+        return made(*a, **k)
+    monkeypatch.setattr(eng, "_new_request", new_request)
+
+    def end():
+        thread.join(30)
+        assert not thread.is_alive()
+        return refused
+    return end
+
+
+@pytest.mark.parametrize("limits", [(4, 40), (40, 4), (4, 4, 40)])
+def test_a_smaller_pool_and_continuations_of_several_lengths(monkeypatch, limits):
+    """Either the pool is smaller and the continuations are refused, or they are there and the smaller pool is: never both."""
+    d, _ = driver(max_num_seqs=4, max_model_len=64, block_size=4, num_blocks=16)
+    end = resized_on_the_way(monkeypatch, d, 3)
+    params = [SamplingParams(max_new_tokens=n, seed=i) for i, n in enumerate(limits)]
+    try:
+        ids = add_continuations(d, [1, 2, 3], len(limits), params)
+    except ValueError:
+        end()
+        assert not d.requests and not d.router._queues and not has_work(d)
+        return
+    reqs = [d.requests[i] for i in ids]
+    assert end() and d.cache.num_pages == 16           # the continuations came first
+    while has_work(d):
+        step(d)
+        d.cache.check()
+    assert [r.output_ids for r in reqs] == [expected([1, 2, 3], n, i) for i, n in enumerate(limits)]
+
+
+def test_a_smaller_pool_and_a_request(monkeypatch):
+    d, _ = driver(max_num_seqs=2, max_model_len=64, block_size=4, num_blocks=16)
+    end = resized_on_the_way(monkeypatch, d, 3)
+    try:
+        i = add_request(d, [1, 2, 3], SamplingParams(max_new_tokens=40, seed=0))
+    except ValueError:
+        end()
+        assert not d.requests and not d.router._queues and not has_work(d)
+        return
+    req = d.requests[i]
+    assert end()
+    while has_work(d):
+        step(d)
+    assert req.output_ids == expected([1, 2, 3], 40, 0)
+
+
+def test_what_is_refused_leaves_nothing_behind():
+    """A pool that became too small before the request was made."""
+    d, _ = driver(max_num_seqs=2, max_model_len=64, block_size=4, num_blocks=16)
+    resize_cache(d, 3)
+    for call in (lambda: add_request(d, [1], SamplingParams(max_new_tokens=40)),
+                 lambda: add_continuations(d, [1], 2, [SamplingParams(max_new_tokens=4), SamplingParams(max_new_tokens=40)])):
+        with pytest.raises(ValueError, match="pages"):
+            call()
+        assert not d.requests and not d.router._queues and not has_work(d)
