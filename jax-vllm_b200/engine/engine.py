@@ -237,6 +237,11 @@ def _step_locked(driver: Driver) -> list:
     sched = driver.scheduler
     if driver.cache.broken:
         raise RuntimeError(driver.cache.broken)
+    # A step that samples ends with the host waiting for its tokens.  What does not (a step without logits, copies for forks)
+    # may still run when the next one is issued, by another thread or on another stream.
+    leave, follow = getattr(driver.runner, "leave", None), getattr(driver.runner, "follow", None)
+    if follow is not None:
+        follow()
     ahead, driver.ahead = driver.ahead, None
     plan = sched.take_ahead(ahead) or sched.schedule()
     if not plan:
@@ -271,6 +276,8 @@ def _step_locked(driver: Driver) -> list:
         st.max_pages_in_use = max(st.max_pages_in_use, st.pages_in_use)
     events: list = []
     if not sampled:
+        if leave is not None:
+            leave()
         return events
     if both is None:
         parts = [[], [], [], []]
@@ -353,6 +360,8 @@ def _step_locked(driver: Driver) -> list:
             sched.fork(s.request, go_on)
         if made[0][1].finished:
             sched.finish(s.request)
+    if forking and leave is not None:
+        leave()
     return events
 
 

@@ -80,6 +80,7 @@ class Runner:
         self.layer_caches = [views.get(k) for k in range(len(model.order))]
         self.builder = BatchBuilder(len(cache.groups), cache.page_size, model.tile_classes(cache.page_size), self.device)
         self.steps = 0
+        self._left = None                  # an event behind work on the cache that nobody has waited for
 
     @torch.no_grad()
     def step(self, entries: list) -> torch.Tensor:
@@ -99,6 +100,20 @@ class Runner:
                     logits = self.model.forward(ctx, self.layer_caches)
         self.steps += 1
         return logits
+
+    def leave(self) -> None:
+        """Work on the cache goes on, on the caller's stream, after the caller has returned: `follow` orders what comes next."""
+        self._left = torch.cuda.Event()
+        self._left.record(torch.cuda.current_stream(self.device))
+
+    def follow(self) -> None:
+        """What the caller issues from here on, on whatever stream it has, follows the work that was left running."""
+        if self._left is None:
+            return
+        if self._left.query():
+            self._left = None
+        else:
+            torch.cuda.current_stream(self.device).wait_event(self._left)
 
     # ----------------------------------------------------------- captured decode steps
     def _graphable(self, entries) -> bool:

@@ -80,3 +80,26 @@ def test_what_is_refused_leaves_nothing_behind():
         with pytest.raises(ValueError, match="pages"):
             call()
         assert not d.requests and not d.router._queues and not has_work(d)
+
+
+# ------------------------------------------------------------------------------------------------------ work in flight
+@pytest.mark.parametrize("n", [1, 3])
+def test_the_next_step_follows_what_a_step_leaves_running(n):
+    """A portion of a prompt without logits, and the copies for forks, are not waited for: the runner is told, after them, and
+    asked to follow them before anything else is issued."""
+    d, r = driver(max_num_seqs=4, max_model_len=64, block_size=4, max_tokens_per_step=8)
+    log = []
+    r.leave, r.follow = lambda: log.append("leave"), lambda: log.append("follow")
+    run, fork, admit = r.step, d.cache.fork, d.cache.admit
+    r.step = lambda entries: log.append("step") or run(entries)
+    d.cache.fork = lambda *a: log.append("fork") or fork(*a)
+    d.cache.admit = lambda *a: log.append("admit") or admit(*a)          # clears state rows on the device
+    add_continuations(d, [5] * 13, n, SamplingParams(max_new_tokens=4, seed=0))
+    step(d)                                            # eight tokens of the prompt
+    assert log == ["follow", "admit", "step", "leave"]
+    del log[:]
+    step(d)                                            # the rest, and the first tokens
+    assert log == ["follow", "step"] + (["fork", "leave"] if n > 1 else [])
+    del log[:]
+    step(d)
+    assert log == ["follow", "step"]

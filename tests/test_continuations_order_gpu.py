@@ -1,0 +1,59 @@
+"""Steps, forks and sizes on several streams and from several threads on the GPU: the tokens of one stream and one thread."""
+
+import pytest
+import torch
+
+from tests.util import PAGE_SIZE, TINY, make_folder, random_tokens
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def model(tmp_path_factory):
+    from jax_vllm_b200 import load_from_path
+    return load_from_path(make_folder(tmp_path_factory.mktemp("order"), "a", seed=6), dtype="fp32")
+
+
+P, VOCAB = PAGE_SIZE["a"], TINY["a"]["vocab_size"]
+
+
+def driver(model, **kw):
+    from jax_vllm_b200 import make_driver
+    return make_driver(model, **{**dict(max_num_seqs=5, max_model_len=96, block_size=P), **kw})
+
+
+def params(n, length=12):
+    from jax_vllm_b200 import SamplingParams
+    return [SamplingParams(max_new_tokens=length, temperature=0.9, top_p=0.95, seed=300 + i) for i in range(n)]
+
+
+@pytest.mark.parametrize("portions", [False, True], ids=["whole prompt", "in portions"])
+def test_steps_on_streams_in_turn(model, portions):
+    """Every step on another stream than the last; each stream is busy (20 million clocks, 10 ms) before it gets to the step's
+    last work, so that nothing but the engine's own order keeps the next step behind it."""
+    from jax_vllm_b200 import add_continuations, continuations, has_work, step
+    prompt = random_tokens(2 * P + 3, VOCAB, seed=41)
+    kw = dict(max_tokens_per_step=P + 1) if portions else {}
+    want = [r.output_ids for r in continuations(driver(model, **kw), prompt, 4, params(4))]
+    d = driver(model, **kw)
+    fork, run = d.cache.fork, d.runner.step
+
+    def late_fork(*a):
+        torch.cuda._sleep(20_000_000)
+        return fork(*a)
+
+    def late_step(entries):
+        if portions:
+            torch.cuda._sleep(20_000_000)
+        return run(entries)
+    d.cache.fork, d.runner.step = late_fork, late_step
+    reqs = [d.requests[i] for i in add_continuations(d, prompt, 4, params(4))]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    k = 0
+    while has_work(d):
+        with torch.cuda.stream(streams[k % 3]):
+            step(d)
+        k += 1
+    assert d.stats.forks == 3
+    assert [r.output_ids for r in reqs] == want
