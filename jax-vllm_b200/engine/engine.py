@@ -154,6 +154,13 @@ def add_continuations(driver: Driver, prompt_ids, n: int, sampling=None) -> list
     return _add(driver, _checked_prompt(driver, prompt_ids), sampling)
 
 
+def _order(driver: Driver) -> tuple:
+    """(leave, follow) of the runner: a step that samples ends with the host waiting for its tokens, but what does not (a step
+    without logits, copies for forks) may still run when the next one is issued, by another thread or on another stream."""
+    nothing = lambda: None  # noqa: E731
+    return getattr(driver.runner, "leave", nothing), getattr(driver.runner, "follow", nothing)
+
+
 @contextlib.contextmanager
 def _device_idle(driver: Driver):
     """What is done to the cache between two steps, on whatever stream the caller has, begins after the steps issued so far
@@ -186,8 +193,11 @@ def fork_request(driver: Driver, request_id: int, sampling: Optional[SamplingPar
         child = _new_request(driver, parent.prompt_ids, sp)
         child.output_ids = list(parent.output_ids)
         driver.requests[child.request_id] = child
-        with _device_idle(driver):
-            driver.scheduler.fork(parent, [child])
+        # the copies follow the last step, and the next step follows them: nothing else on the device is waited for
+        leave, follow = _order(driver)
+        follow()
+        driver.scheduler.fork(parent, [child])
+        leave()
     driver.router.wake()
     return child.request_id
 
@@ -237,11 +247,8 @@ def _step_locked(driver: Driver) -> list:
     sched = driver.scheduler
     if driver.cache.broken:
         raise RuntimeError(driver.cache.broken)
-    # A step that samples ends with the host waiting for its tokens.  What does not (a step without logits, copies for forks)
-    # may still run when the next one is issued, by another thread or on another stream.
-    leave, follow = getattr(driver.runner, "leave", None), getattr(driver.runner, "follow", None)
-    if follow is not None:
-        follow()
+    leave, follow = _order(driver)
+    follow()
     ahead, driver.ahead = driver.ahead, None
     plan = sched.take_ahead(ahead) or sched.schedule()
     if not plan:
@@ -276,8 +283,7 @@ def _step_locked(driver: Driver) -> list:
         st.max_pages_in_use = max(st.max_pages_in_use, st.pages_in_use)
     events: list = []
     if not sampled:
-        if leave is not None:
-            leave()
+        leave()
         return events
     if both is None:
         parts = [[], [], [], []]
@@ -360,7 +366,7 @@ def _step_locked(driver: Driver) -> list:
             sched.fork(s.request, go_on)
         if made[0][1].finished:
             sched.finish(s.request)
-    if forking and leave is not None:
+    if forking:
         leave()
     return events
 

@@ -4,7 +4,7 @@ import threading
 
 import pytest
 
-from jax_vllm_b200.engine import SamplingParams, add_continuations, add_request, has_work, resize_cache, step
+from jax_vllm_b200.engine import SamplingParams, add_continuations, add_request, fork_request, has_work, resize_cache, step
 from jax_vllm_b200.engine import engine as eng
 from tests.test_continuations import driver, expected
 
@@ -103,3 +103,15 @@ def test_the_next_step_follows_what_a_step_leaves_running(n):
     del log[:]
     step(d)
     assert log == ["follow", "step"]
+
+
+def test_a_fork_between_steps_is_ordered_like_a_step():
+    d, r = driver(max_num_seqs=4, max_model_len=64, block_size=4)
+    a = add_request(d, [5] * 6, SamplingParams(max_new_tokens=6, seed=0))
+    step(d)
+    log = []
+    r.leave, r.follow = lambda: log.append("leave"), lambda: log.append("follow")
+    fork = d.cache.fork
+    d.cache.fork = lambda *a: log.append("fork") or fork(*a)
+    fork_request(d, a)
+    assert log == ["follow", "fork", "leave"]

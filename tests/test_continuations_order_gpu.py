@@ -57,3 +57,26 @@ def test_steps_on_streams_in_turn(model, portions):
         k += 1
     assert d.stats.forks == 3
     assert [r.output_ids for r in reqs] == want
+
+
+def test_a_fork_waits_for_nothing_but_the_cache(model):
+    """A request is forked while a stream that has nothing to do with the engine is busy (a second or so): the call returns
+    before that has ended, and the fork's tokens are the ones that it has to give."""
+    from jax_vllm_b200 import add_request, fork_request, has_work, step
+    prompt = random_tokens(P + 3, VOCAB, seed=43)
+    d = driver(model)
+    a = add_request(d, prompt, params(1)[0])
+    for _ in range(4):
+        step(d)
+    torch.cuda.synchronize()
+    other, side, done = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.Event()
+    with torch.cuda.stream(other):
+        torch.cuda._sleep(1_500_000_000)
+        done.record()
+    with torch.cuda.stream(side):
+        b = fork_request(d, a, params(1)[0])
+    assert not done.query()
+    reqs = [d.requests[i] for i in (a, b)]
+    while has_work(d):
+        step(d)
+    assert reqs[0].output_ids == reqs[1].output_ids and d.stats.forks == 1
