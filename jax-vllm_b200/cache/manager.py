@@ -345,7 +345,7 @@ class CacheManager:
         anything has changed; should an allocation fail all the same, the cache is `broken` and takes no more steps."""
         if num_pages < 1:
             raise ValueError("a pool needs at least one page")
-        self._check_room(num_pages)
+        self.check_room(num_pages)
         pools = [grp.pool.resized(num_pages) for grp in self.groups]
         try:
             self._move(num_pages, pools)
@@ -356,8 +356,10 @@ class CacheManager:
     def _stores(self) -> list:
         return [t for grp in self.groups for t in ((grp.k,) if grp.v is grp.k else (grp.k, grp.v)) if t is not None]
 
-    def _check_room(self, num_pages: int) -> None:
-        """Refuses new stores that would not fit beside the old ones that are left when each is allocated."""
+    def check_room(self, num_pages: int, captured: bool = False) -> None:
+        """Refuses new stores that would not fit beside the old ones that are left when each is allocated.  With `captured`,
+        steps that are captured now will have been dropped by then: what the allocator has reserved for them, and no tensor
+        holds, counts as free."""
         extra = most = 0
         for old in self._stores():
             new = old.nbytes // old.shape[1] * num_pages
@@ -367,6 +369,8 @@ class CacheManager:
         if device is not None and device.type == "cuda":
             torch.cuda.empty_cache()             # what no tensor holds goes back to the device, so that it counts as free
             free = torch.cuda.mem_get_info(device)[0]
+            if captured:
+                free += torch.cuda.memory_reserved(device) - torch.cuda.memory_allocated(device)
             if most > free:
                 raise ValueError(f"{num_pages} pages need {most} bytes of device memory while they take over the old ones, {free} are free")
 

@@ -220,6 +220,7 @@ def resize_cache(driver: Driver, num_blocks: int) -> None:
         held = max(cache.num_pages - g.pool.num_free for g in cache.groups)
         if num_blocks < max(1, held):
             raise ValueError(f"{held} pages are in use, {num_blocks} were asked for")
+        cache.check_room(num_blocks, captured=True)      # what is refused costs no captured step
         driver.ahead = None
         if hasattr(driver.runner, "forget_graphs"):
             driver.runner.forget_graphs()

@@ -3,6 +3,7 @@
 import threading
 
 import pytest
+import torch
 
 from jax_vllm_b200.engine import SamplingParams, add_continuations, add_request, fork_request, has_work, resize_cache, step
 from jax_vllm_b200.engine import engine as eng
@@ -115,3 +116,35 @@ def test_a_fork_between_steps_is_ordered_like_a_step():
     d.cache.fork = lambda *a: log.append("fork") or fork(*a)
     fork_request(d, a)
     assert log == ["follow", "fork", "leave"]
+
+
+# --------------------------------------------------------------------------------------------------------------- sizes
+def test_a_size_that_is_refused_costs_no_captured_step(monkeypatch):
+    """Too small for what is live, too large for the device: both before the runner drops its captured steps."""
+    d, r = driver(max_num_seqs=2, max_model_len=64, block_size=4, num_blocks=16)
+    forgotten = []
+    r.forget_graphs = lambda: forgotten.append(d.cache.num_pages)
+    add_request(d, [1, 2, 3], SamplingParams(max_new_tokens=20, seed=0))
+    step(d)
+    ahead = d.ahead
+    with pytest.raises(ValueError):
+        resize_cache(d, 3)
+    device = torch.device("cuda")
+    monkeypatch.setattr(type(d.cache), "_stores", lambda self: [FakeStore(device, 1 << 20, 16)])
+    monkeypatch.setattr(torch.cuda, "empty_cache", lambda: None)
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device: (5 << 20, 9 << 20))
+    monkeypatch.setattr(torch.cuda, "memory_reserved", lambda device: 3 << 20)
+    monkeypatch.setattr(torch.cuda, "memory_allocated", lambda device: 1 << 20)
+    with pytest.raises(ValueError, match="device memory"):
+        resize_cache(d, 16 * 8)                        # 8 MB; 5 are free and 2 more without captured steps
+    assert not forgotten and d.ahead is ahead and d.cache.num_pages == 16
+    with pytest.raises(ValueError, match="device memory"):
+        resize_cache(d, 16 * 6)                        # 6 MB: they go, and leave no more than before here
+    assert forgotten == [16] and d.cache.num_pages == 16 and d.cache.broken is None
+
+
+class FakeStore:
+    """What the check of the room asks of a store."""
+
+    def __init__(self, device, nbytes, pages):
+        self.device, self.nbytes, self.shape = device, nbytes, (1, pages)

@@ -80,3 +80,21 @@ def test_a_fork_waits_for_nothing_but_the_cache(model):
     while has_work(d):
         step(d)
     assert reqs[0].output_ids == reqs[1].output_ids and d.stats.forks == 1
+
+
+def test_a_refused_size_keeps_the_captured_steps(model):
+    from jax_vllm_b200 import generate, resize_cache
+    d = driver(model, num_blocks=40)
+    prompts = [random_tokens(n, VOCAB, seed=50 + n) for n in (5, 9)]
+    want = generate(d, prompts, params(2))
+    kept = {n: g for n, g in d.runner.graphs_filtered.items()}
+    assert kept
+    page = sum(t.nbytes for g in d.cache.groups for t in (g.k, g.v)) // 40
+    for size in (0, (1 << 39) // page):                # none, and three times what the device has
+        with pytest.raises(ValueError):
+            resize_cache(d, size)
+    assert d.runner.graphs_filtered == kept
+    assert generate(d, prompts, params(2)) == want
+    resize_cache(d, 41)
+    assert not d.runner.graphs_filtered
+    assert generate(d, prompts, params(2)) == want
