@@ -419,8 +419,9 @@ def stop(driver: Driver, join: bool = True) -> None:
 
 def prewarm(driver: Driver) -> float:
     """Compiles what the model needs, runs one tiny batch and captures the decode graphs of every batch size up
-    to `max_num_seqs`, so that no request pays for it (the reference compiles its shape buckets here,
-    jllm/engine/engine.py:112-150).  Returns the seconds it took."""
+    to `max_num_seqs`, without filters and with them, so that no request pays for it (the reference compiles its
+    shape buckets here, jllm/engine/engine.py:112-150); steps that give log-probabilities are captured when they
+    are first needed.  Returns the seconds it took."""
     t0 = time.perf_counter()
     with driver.step_lock:
         driver.ahead = None

@@ -298,8 +298,10 @@ class Runner:
 
     def warm_up(self, decode_batches: int = 0) -> None:
         """One two-token portion and one single token through every kernel of the model; then, with CUDA
-        graphs, the decode steps of 1 .. `decode_batches` requests with their sampling are captured (a step
-        of each size runs twice: once eagerly, once into the graph), so that no request pays for that."""
+        graphs, the decode steps of 1 .. `decode_batches` requests with their sampling, without filters and with
+        them, are captured (a step of each size runs eagerly once, then into the graphs), so that no request
+        pays for that.  Steps that give log-probabilities are captured when they are first needed: their graphs
+        keep the logits of every batch size."""
         if not self.cache.can_admit():
             return
         rc = self.cache.admit("__warm_up__")
@@ -326,10 +328,12 @@ class Runner:
                 self.cache.grow(rc, 2)
                 rc.num_tokens = 1              # as if one token were cached: the step adds the second
                 entries = [StepEntry(r, [0], (0,)) for r in live]
-                zeros = [0.0] * n
-                if self.step_sampled(entries, zeros, [0] * n, [0] * n) is None:
+                draws = [[0.0] * n, [0] * n, [0] * n]
+                if self.step_sampled(entries, *draws) is None:
                     self.step(entries)                                       # the first time at this size: eagerly
-                    self.step_sampled(entries, zeros, [0] * n, [0] * n)      # then into the graph
+                    self.step_sampled(entries, *draws)                       # then into the graph
+                if self.model.spec.vocab_size <= ops.MOST_VOCAB:
+                    self.step_sampled(entries, *draws, [(0, 1.0, 0.0)] * n)
             self.check_kernels()
         finally:
             for r in live:

@@ -98,3 +98,17 @@ def test_a_refused_size_keeps_the_captured_steps(model):
     resize_cache(d, 41)
     assert not d.runner.graphs_filtered
     assert generate(d, prompts, params(2)) == want
+
+
+def test_prewarming_captures_the_steps_with_filters_too(model):
+    from jax_vllm_b200 import generate, prewarm
+    prompts = [random_tokens(n, VOCAB, seed=60 + n) for n in (5, 19, 2)]
+    want = generate(driver(model, max_num_seqs=3), prompts, params(3))
+    d = driver(model, max_num_seqs=3)
+    prewarm(d)
+    assert sorted(d.runner.graphs_sampled) == sorted(d.runner.graphs_filtered) == [1, 2, 3]
+    d.cache.check()
+    assert not d.cache.live
+    kept = dict(d.runner.graphs_filtered)
+    assert generate(d, prompts, params(3)) == want
+    assert d.runner.graphs_filtered == kept and d.runner.graph_replays > 10
