@@ -2664,6 +2664,25 @@ def _span(t: torch.Tensor) -> tuple:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two stores [layers, pages, page...] have a page in common, or parts of one (stores of different strides: whether
+    the memory between their ends meets)."""
+    first, last = _span(a)
+    other, end = _span(b)
+    if first >= end or other >= last:
+        return False
+    if a.stride()[:2] != b.stride()[:2]:
+        return True
+    size = a.element_size()
+    layer, page, row, apart = a.stride(0) * size, a.stride(1) * size, math.prod(a.shape[2:]) * size, other - first
+    for k in range(1 - a.shape[0], b.shape[0]):
+        near = -(apart + k * layer) // page if page else 0
+        for p in (near, near + 1):
+            if abs(apart + k * layer + min(max(p, 1 - a.shape[1]), b.shape[1] - 1) * page) < row:
+                return True
+    return False
+
+
 _PAGE_COPY_TYPES = [c_char_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p]
 
 
@@ -2699,7 +2718,8 @@ def copy_pages(stores, src, dst, tokens=None, into=None) -> None:
     of the store at the same place of `into` (a pool of another size).  src and dst are integers on the host; no page is
     given twice as a destination, and in place none is both source and destination.  `tokens[i]` copies only the first
     so many tokens of the page; what follows them in the destination stays as it was.  A store may have any strides over
-    layers and pages; a page itself is contiguous.  The stores of `into` lie apart in memory from those that are read."""
+    layers and pages; a page itself is contiguous.  The stores of a list lie apart in memory (keys and values may be parts of
+    one tensor), those of `into` from those that are read too."""
     stores = list(stores)
     to = stores if into is None else list(into)
     if not stores or len(to) != len(stores):
@@ -2723,20 +2743,23 @@ def copy_pages(stores, src, dst, tokens=None, into=None) -> None:
             planes += (a.data_ptr(), b.data_ptr(), layer * size, page * size, to_layer * size, to_page * size, row * size, row // page_size * size,
                        shape[0])
     pairs = check_copies("copy_pages", src, dst, n_src, n_dst, into is not None, tokens, page_size)
-    for a in stores:
-        _on_current_device("copy_pages", a.get_device())
     if into is not None:
         spans = [_span(t) for t in to if t.numel()]
         for x in (_span(t) for t in stores if t.numel()):
             if any(x[0] < y[1] and y[0] < x[1] for y in spans):
                 raise KernelError("copy_pages: the stores to copy into must lie apart from the others in memory")
+        if any(_meet(a, b) for k, a in enumerate(to) for b in to[:k] if a.numel() and b.numel()):
+            raise KernelError("copy_pages: the stores to copy into must lie apart from one another in memory")
+    for a in stores:
+        _on_current_device("copy_pages", a.get_device())
     if pairs[0] and planes:
         _copy_planes("copy_pages", planes, pairs)
 
 
 def copy_slots(states, src, dst) -> None:
     """Copies rows of per-request state: row src[i] of every tensor [slots, ...] to row dst[i] of the same tensor, under the
-    rules of `copy_pages`.  The tensors may have different shapes behind the slots, and different types."""
+    rules of `copy_pages`.  The tensors may have different shapes behind the slots, and different types; they lie apart in
+    memory."""
     states = list(states)
     if not states:
         raise KernelError("copy_slots: a list of state tensors")
