@@ -154,6 +154,12 @@ def add_continuations(driver: Driver, prompt_ids, n: int, sampling=None) -> list
     return _add(driver, _checked_prompt(driver, prompt_ids), sampling)
 
 
+def _on_device(driver: Driver):
+    """The driver's device as the current one: launches, events and copies go to the current device's stream."""
+    device = torch.device(driver.config.device)
+    return torch.cuda.device(device) if device.type == "cuda" else contextlib.nullcontext()
+
+
 def _order(driver: Driver) -> tuple:
     """(leave, follow) of the runner: a step that samples ends with the host waiting for its tokens, but what does not (a step
     without logits, copies for forks) may still run when the next one is issued, by another thread or on another stream."""
@@ -180,7 +186,7 @@ def fork_request(driver: Driver, request_id: int, sampling: Optional[SamplingPar
     again.  Its tokens so far are the other's, its events those that it produces itself; `max_new_tokens` counts both.
     `sampling` defaults to the other's parameters, without a seed."""
     driver.router.raise_if_failed()
-    with driver.step_lock:
+    with driver.step_lock, _on_device(driver):
         parent = driver.requests.get(request_id)
         if parent is None or parent.finished:
             raise KeyError(f"request {request_id} is not running")
@@ -208,7 +214,7 @@ def resize_cache(driver: Driver, num_blocks: int) -> None:
     finished could need more pages than there would be.  The captured decode steps are dropped and captured again when
     they are next needed."""
     driver.router.raise_if_failed()
-    with driver.step_lock:
+    with driver.step_lock, _on_device(driver):
         cache, sched = driver.cache, driver.scheduler
         if not cache.groups:
             raise ValueError("the model keeps no pages")
@@ -240,7 +246,7 @@ def has_work(driver: Driver) -> bool:
 def step(driver: Driver) -> list:
     """One scheduler iteration: at most one batch on the device; returns its StepEvents."""
     driver.router.raise_if_failed()
-    with driver.step_lock:
+    with driver.step_lock, _on_device(driver):
         return _step_locked(driver)
 
 

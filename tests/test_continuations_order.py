@@ -148,3 +148,37 @@ class FakeStore:
 
     def __init__(self, device, nbytes, pages):
         self.device, self.nbytes, self.shape = device, nbytes, (1, pages)
+
+
+def test_what_the_entry_point_issues_goes_to_the_driver_s_device(monkeypatch):
+    """A driver of the second GPU, used while the first is the current one (both stand-ins): the runner, the sampler, the copies
+    of forks and of a resize all find the driver's device current."""
+    d, r = driver(max_num_seqs=4, max_model_len=64, block_size=4)
+    current, seen = ["cuda:0"], []
+
+    class Device:
+        def __init__(self, device):
+            self.device = str(device)
+
+        def __enter__(self):
+            current.append(self.device)
+
+        def __exit__(self, *a):
+            current.pop()
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: None)
+    monkeypatch.setattr(torch.cuda, "empty_cache", lambda: None)
+    object.__setattr__(d.config, "device", "cuda:1")
+
+    def watched(owner, name):
+        call = getattr(owner, name)
+        setattr(owner, name, lambda *a: seen.append((name, current[-1])) or call(*a))
+    for owner, name in ((r, "step"), (d.sampler, "sample"), (d.cache, "fork"), (d.cache, "resize")):
+        watched(owner, name)
+    add_continuations(d, [5] * 6, 2, SamplingParams(max_new_tokens=6, seed=0))
+    step(d)
+    fork_request(d, 0)
+    resize_cache(d, d.num_blocks + 1)
+    step(d)
+    assert [name for name, _ in seen] == ["step", "sample", "fork", "fork", "resize", "step", "sample"]
+    assert {device for _, device in seen} == {"cuda:1"} and current == ["cuda:0"]
