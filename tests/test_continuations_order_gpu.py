@@ -1,5 +1,8 @@
 """Steps, forks and sizes on several streams and from several threads on the GPU: the tokens of one stream and one thread."""
 
+import random
+import threading
+
 import pytest
 import torch
 
@@ -112,3 +115,47 @@ def test_prewarming_captures_the_steps_with_filters_too(model):
     kept = dict(d.runner.graphs_filtered)
     assert generate(d, prompts, params(3)) == want
     assert d.runner.graphs_filtered == kept and d.runner.graph_replays > 10
+
+
+def test_continuations_of_several_lengths_from_several_threads(model):
+    """Threads that add continuations with limits of their own, fork them and change the pool's size while the engine's thread
+    steps (a size that is too small for what is live is refused).  Every token is that of the request alone."""
+    from jax_vllm_b200 import SamplingParams, add_continuations, fork_request, generate, resize_cache, start, stop, stream
+    prompts = [random_tokens(n, VOCAB, seed=70 + n) for n in (3, P, 2 * P + 1)]
+    limits = (4, 30, 11)
+    sp = lambda k, i: SamplingParams(max_new_tokens=limits[(k + i) % 3], temperature=0.9, top_k=30, top_p=0.95, seed=1000 * k + i)  # noqa: E731
+    alone = driver(model, max_num_seqs=1)
+    want = {(k, i): generate(alone, [prompts[k % 3]], sp(k, i))[0] for k in range(4) for i in range(3)}
+    d = driver(model, num_blocks=40)
+    faults = []
+
+    def work(k):
+        r = random.Random(k)
+        try:
+            for _ in range(3):
+                ids = add_continuations(d, prompts[k % 3], 3, [sp(k, i) for i in range(3)])
+                try:
+                    f = fork_request(d, ids[0], sp(k, 0))
+                    got = [e.token for e in stream(d, f)]
+                    assert got == want[k, 0][len(want[k, 0]) - len(got):]
+                except (KeyError, ValueError):         # it has finished, or has as many tokens as it may
+                    pass
+                try:
+                    resize_cache(d, r.randrange(5, 60))
+                except ValueError:                     # too few pages for what is live
+                    pass
+                for i, rid in enumerate(ids):
+                    assert [e.token for e in stream(d, rid)] == want[k, i]
+        except BaseException as exc:
+            faults.append(exc)
+
+    start(d)
+    threads = [threading.Thread(target=work, args=(k,), daemon=True) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not faults and not any(t.is_alive() for t in threads) and d.router.failure is None
+    stop(d)
+    d.cache.check()
+    assert not d.cache.live and not d.requests
