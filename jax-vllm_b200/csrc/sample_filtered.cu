@@ -7,7 +7,12 @@
 //                softmax over it that depends on the row's own numbers only, as in sampling.cu and with its arithmetic
 //   T == 0       the largest logit
 // Every filter leaves the first tokens up to a boundary, so the kept ones are a range of the composed numbers of
-// vocab_row.h, and only they need a random number.  Tokens with (largest - x) / T > 30 are left out from the start where
+// vocab_row.h, and only they need a random number.  Counts and shares have exact boundaries, the same in every batch.  The
+// boundary of a mass is a comparison of sums, 32-bit within a thread (columns of 64 bits would fill the shared memory of a
+// multiprocessor with one block); which logits a thread adds follows the number of blocks that read the row, hence the number of rows,
+// and the row's place beside 16-byte boundaries.  So a token whose border lies within the rounding of the sums (6e-5 of the mass at
+// most, about 2e-8 as restated on the host) may be kept in one batch and left out in another: none of 10,240 even rows of
+// 32,003 logits drew another token with eight blocks than with one.  Tokens with (largest - x) / T > 30 are left out from the start where
 // there is a filter: their mass is below 1e-13 of the largest's, and -log(-log(u)) lies between -2.9 and 16.7, so that they
 // cannot be drawn before the largest.
 //

@@ -3,7 +3,8 @@
 // The tokens of a row are in order of their logits, the lowest index first among equal ones.  Both are one number,
 //   c = key(x) << 20 | (2^20 - 1 - index),     key: the bits of x, made to ascend with x
 // so that "the first tokens up to some boundary" are the tokens with c >= cut.  A NaN counts as minus infinity and -0 as 0.
-// A token weighs exp((x - largest) / T) in 32 bits; sums are 32-bit within a thread, 64-bit across threads, in a fixed order.
+// A token weighs exp((x - largest) / T) in 32 bits; sums are 32-bit within a thread, 64-bit across threads, in an order that follows
+// the row's length, its place beside 16-byte boundaries and the number of blocks that read it.
 //
 // Few first tokens are found in two passes.  In the first every thread keeps its largest logit.  The j-th largest of a block's
 // (of its warps, of 128 groups of four threads, or of the threads where j is large) has at least j tokens at or above it in that block, and

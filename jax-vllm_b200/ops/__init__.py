@@ -2584,9 +2584,10 @@ def sample_filtered(logits: torch.Tensor, temperature: torch.Tensor, top_k: torc
         min_p > 0            of these, the ones with p >= min_p (more than 1 counts as 1)
         top_p < 1            of these, the ones before which less than top_p of their sum of p lies; the first always
 
-    The draw is the kept token with the largest logit / temperature - log(-log(u)), where u depends on (seed, counter,
-    token id) only: the numbers of `sample`, whose tokens a row without filters gets.  A temperature of 0 takes the largest
-    logit.  A NaN counts as minus infinity; a row with nothing else gives token 0."""
+    The draw is the kept token with the largest logit / temperature - log(-log(u)), where u in (0, 1) depends on (seed, counter,
+    token id) only: the numbers of `sample`, whose tokens a row without filters gets.  top_p compares sums of 32-bit masses, whose
+    order follows the number of rows: a token whose border lies within their rounding may be kept in one batch and not in
+    another.  A temperature of 0 takes the largest logit.  A NaN counts as minus infinity; a row with nothing else gives token 0."""
     rows, vocab, stride, code = _logit_rows("sample_filtered", logits, (
         ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
         ("min_p", min_p, torch.float32), ("seeds", seeds, torch.int64), ("counters", counters, torch.int64)))

@@ -5,7 +5,8 @@ The reference samples greedily only (argmax, jllm/engine/generate.py:142 and
 jllm/engine/state.py:66).  Temperature sampling here is a draw from
 softmax(logits / temperature) whose random numbers are keyed by (seed of the request,
 index of the output token, vocabulary index), so a request's tokens do not depend on the
-batch it is sampled in.
+batch it is sampled in (under top_p: but for a token whose border lies within the rounding
+of 32-bit sums, see ops.sample_filtered).
 """
 
 from __future__ import annotations
