@@ -45,7 +45,9 @@ struct SampleParams {
 };
 
 constexpr float DEEPEST = 30.f;
-constexpr int FIRST_LOOK = 128;                        // tokens that the list is meant to hold where no count says how many
+// Tokens that the list is meant to hold where no count says how many.  (64 rows of 151,936 with 200 peaks under top-p: 21.5 us; a list
+// meant for 64 takes 19.1 where it does and 34 to 41 where it does not, one for 256 takes 22.9.)
+constexpr int FIRST_LOOK = 128;
 constexpr float LOG2E = 1.4426950408889634f;
 
 // The best score so far and its token.
@@ -322,7 +324,9 @@ __device__ __forceinline__ u64 filtered(const SampleParams& p, const Scores& sc,
       mass = sh.part[0][0];
     }
   } else if (can_list && !(summed && largest - sh.bound < 3.f * temp)) {
-    // (of nearly even logits, those from the bound up would hold too little of the mass)
+    // Of nearly even logits, those from the bound up would hold too little of the mass.  (64 rows under top-p: even ones 73.6 us, 81.4
+    // if the list is tried all the same; leaving it out up to 6 T, rows with 200 peaks take 35.5 instead of 21.7, rows of a spread
+    // of 2.2 without peaks 62 instead of 70.)
     if (summed) {
       const float2 q = list_first<T, true>(low, least);
       const double2 a = block_sums((double)q.x, (double)q.y);
@@ -351,6 +355,8 @@ __device__ __forceinline__ u64 filtered(const SampleParams& p, const Scores& sc,
   }
   if (threadIdx.x == 0) sh.listed = 0;
 
+  // The first level's bins: from the largest logit to six times as deep as the bound of few tokens.  (64 even rows: top-p 0.9 73.6 us, with
+  // three times as deep 92.3, with twelve 76.8; the first 1,500 tokens 52.9, 46.5 and 59.2.)
   const float step = DEEPEST * temp, wide = 6.f * (largest - sh.bound);
   const float per = (float)BINS / (wide > 0.f ? fminf(step, wide) : step);
   if (by_count) {                                      // the boundary by count

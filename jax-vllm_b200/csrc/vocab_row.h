@@ -162,8 +162,11 @@ static inline int launch_clusters(void (*kernel)(KArgs...), dim3 grid, dim3 bloc
   return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...) == cudaSuccess ? JV_OK : JV_ERR_LAUNCH;
 }
 
-// Blocks a row: as many as leave two blocks a multiprocessor room at once, while a block has 16 KB of its row or more.  (24 rows
-// of 64 KB: 19.8 us in four blocks each, 22.0 in eight; one row of 608 KB: 10.4 us in eight, 11.5 in four.)
+// Blocks a row: as many as leave two blocks a multiprocessor room at once, while a block has 16 KB of its row or more.  Filtered
+// sampling, us for one, two, four and eight blocks a row: one row of 608 KB 18.0, 13.9, 11.4, 10.5; 24 rows of 64 KB 11.5, 10.8, 10.9, 11.2;
+// 40 rows of 608 KB 19.4, 16.8, 14.1, 20.7; 75 rows 24.7, 19.0, 24.6, 31.6; 128 rows 30.1, 27.4, 33.3, 52.7; 160 rows 31.5, 45.3,
+// 44.4, 63.9; 256 rows 36.6, 52.3, 60.7, 95.6.  Where the device is filled to the last place the next smaller number is the
+// faster one (74 rows: four blocks 24.2, two 16.9; 148 rows: two 31.2, one 28.4).
 static inline int row_blocks(int rows, long long row_bytes) {
   const int room = 2 * jv_multiprocessors();
   int blocks = 1;
@@ -282,7 +285,9 @@ template <typename T> __device__ __noinline__ float my_largest() {
 }
 
 // Whether a list of the tokens from the bound for j tokens a block up is likely to have room: of NT threads with their tokens
-// anywhere, NT * log(NT / (NT - j)) tokens are expected where j threads have one.
+// anywhere, NT * log(NT / (NT - j)) tokens are expected where j threads have one.  A quarter of the list is left for rows that are
+// not as expected.  (The first 1,000 tokens of 64 rows 26.0 us, 49.2 if half is left; the first 200 of 256 rows 58.1 us, which a
+// list that is expected to be full would do in 50.5, and then a row that is not as expected pays for both.)
 __device__ __forceinline__ bool countable(int j, int blocks) {
   return j < NT && (float)(blocks * NT) * -__logf(1.f - (float)j * (1.f / NT)) < 0.75f * LIST;
 }
@@ -460,7 +465,10 @@ template <typename T, bool SUMMED> __device__ __noinline__ float2 put_once(int j
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) raw[u] = left > u * NT ? p[u * NT] : no_vector();
     p += AHEAD * NT;
-    if (k == 0 || k == 3) {                            // what the first vectors hold above their own bound
+    // The bound of the first vectors, and once more when three times as many have been read.  (256
+    // rows with peaks under top-p 46.2 us, 50.3 with the first bound alone, 64.3 with one in every round; rows in ascending order 168,
+    // 166 and 185.)
+    if (k == 0 || k == 3) {
       float g = m;
       if (k == 0) {
 #pragma unroll
@@ -793,6 +801,8 @@ template <bool MASS> __device__ __noinline__ void take_bin(u64 lo, unsigned most
   if (!composed && !enough) {
     const float wide = fminf(to, deepest) - from;
     per = (float)BINS / wide;
+    // (four levels of equal width at most: of logits that are cut off at one value 157 us for 64 rows, two levels 150, seven 189;
+    // of many close to one another and a few far off 96, 98 and 96)
     if (found || depth > 3 || !(wide > 0.f && per > 0.f && per < 1e37f && wide > 1e-6f * fminf(to, deepest))) {
       // the logits crowd, or it is found: a range of composed numbers, of which the parts end with a single one
       const unsigned a = (unsigned)(lo >> INDEX_BITS), z = key_of(largest);
