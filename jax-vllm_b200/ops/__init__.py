@@ -2745,12 +2745,15 @@ def copy_pages(stores, src, dst, tokens=None, into=None) -> None:
                        shape[0])
     pairs = check_copies("copy_pages", src, dst, n_src, n_dst, into is not None, tokens, page_size)
     if into is not None:
-        spans = [_span(t) for t in to if t.numel()]
+        filled = [t for t in to if t.numel()]
+        spans = [_span(t) for t in filled]
         for x in (_span(t) for t in stores if t.numel()):
             if any(x[0] < y[1] and y[0] < x[1] for y in spans):
                 raise KernelError("copy_pages: the stores to copy into must lie apart from the others in memory")
-        if any(_meet(a, b) for k, a in enumerate(to) for b in to[:k] if a.numel() and b.numel()):
-            raise KernelError("copy_pages: the stores to copy into must lie apart from one another in memory")
+        for k, (first, last) in enumerate(spans):
+            for j in range(k):
+                if first < spans[j][1] and spans[j][0] < last and _meet(filled[k], filled[j]):
+                    raise KernelError("copy_pages: the stores to copy into must lie apart from one another in memory")
     for a in stores:
         _on_current_device("copy_pages", a.get_device())
     if pairs[0] and planes:
