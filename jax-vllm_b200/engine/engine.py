@@ -429,7 +429,10 @@ def prewarm(driver: Driver) -> float:
     shape buckets here, jllm/engine/engine.py:112-150); steps that give log-probabilities are captured when they
     are first needed.  Returns the seconds it took."""
     t0 = time.perf_counter()
-    with driver.step_lock:
+    with driver.step_lock, _on_device(driver):
         driver.ahead = None
+        leave, follow = _order(driver)
+        follow()
         driver.runner.warm_up(decode_batches=driver.max_num_seqs)
+        leave()
     return time.perf_counter() - t0

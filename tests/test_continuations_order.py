@@ -5,7 +5,7 @@ import threading
 import pytest
 import torch
 
-from jax_vllm_b200.engine import SamplingParams, add_continuations, add_request, fork_request, has_work, resize_cache, step
+from jax_vllm_b200.engine import SamplingParams, add_continuations, add_request, fork_request, has_work, prewarm, resize_cache, step
 from jax_vllm_b200.engine import engine as eng
 from tests.test_continuations import driver, expected
 
@@ -116,6 +116,15 @@ def test_a_fork_between_steps_is_ordered_like_a_step():
     d.cache.fork = lambda *a: log.append("fork") or fork(*a)
     fork_request(d, a)
     assert log == ["follow", "fork", "leave"]
+
+
+def test_prewarming_is_ordered_like_a_step():
+    d, r = driver(max_num_seqs=2, max_model_len=64, block_size=4)
+    log = []
+    r.leave, r.follow = lambda: log.append("leave"), lambda: log.append("follow")
+    r.warm_up = lambda decode_batches: log.append(("warm", decode_batches))
+    prewarm(d)
+    assert log == ["follow", ("warm", 2), "leave"]
 
 
 # --------------------------------------------------------------------------------------------------------------- sizes
