@@ -8,8 +8,8 @@
 // its first read).  A warp takes one piece of PIECE bytes at a time, 16 bytes a lane and eight loads in flight before the
 // first store, so that the few pieces of a single page still spread over many multiprocessors.  The pairs travel as
 // parameters of the launch: no copy to the device, no workspace, and a captured launch keeps its own.
-// 1,500 pages of 28 layers (5.5 GB moved) in 855 us, 6.44 TB/s; 64 pages of 36 layers 50 us, 6.0 TB/s; one page of 36 layers to
-// three others 3.5 us, of which 0.9 are bytes; eight rows of 24 state tensors to three others each 69 us, 5.8 TB/s.
+// 1,500 pages of 28 layers (5.5 GB moved) in 860 us, 6.40 TB/s; 64 pages of 36 layers 50 us, 6.0 TB/s; one page of 36 layers to
+// three others 3.3 us, of which 0.9 are bytes; eight rows of 24 state tensors to three others each 69 us, 5.8 TB/s.
 #include "common.cuh"
 
 namespace {

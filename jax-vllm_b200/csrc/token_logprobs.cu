@@ -2,7 +2,7 @@
 //   logprob(v) = x_v - largest - log(sum_w exp(x_w - largest))
 // in one pass over the row, with the running largest logit and the sum relative to it in every thread (32 bits), joined in a
 // fixed order.  The `top` likeliest tokens (equal ones in the order of their indices) are found as in vocab_row.h.
-// Bound by memory where rows are many: 1,024 of 151,936 logits in 95.2 us, 6.53 TB/s.  Eight rows 5.4 us: one pass of a cluster of
+// Bound by memory where rows are many: 1,024 of 151,936 logits in 95.6 us, 6.51 TB/s.  Eight rows 5.4 us: one pass of a cluster of
 // eight blocks and a barrier.  With likely tokens a second pass and a sort (64 rows of 50,021 16-bit logits, 20 tokens: 10.7 us).
 // A NaN counts as minus infinity; a row that holds nothing else has no likely tokens (every logprob is minus infinity);
 // where the largest logit is infinite, the infinite ones share the probability.
