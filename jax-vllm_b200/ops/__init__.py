@@ -2672,14 +2672,17 @@ def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     other, end = _span(b)
     if first >= end or other >= last:
         return False
-    if a.stride()[:2] != b.stride()[:2]:
+    size, other_size = a.element_size(), b.element_size()
+    layer, page = a.stride(0) * size, a.stride(1) * size
+    if (layer, page) != (b.stride(0) * other_size, b.stride(1) * other_size):
         return True
-    size = a.element_size()
-    layer, page, row, apart = a.stride(0) * size, a.stride(1) * size, math.prod(a.shape[2:]) * size, other - first
+    row, other_row = math.prod(a.shape[2:]) * size, math.prod(b.shape[2:]) * other_size
     for k in range(1 - a.shape[0], b.shape[0]):
-        near = -(apart + k * layer) // page if page else 0
+        base = other - first + k * layer                  # from a page of one store to a page of the other, k layers on
+        near = -base // page if page else 0
         for p in (near, near + 1):
-            if abs(apart + k * layer + min(max(p, 1 - a.shape[1]), b.shape[1] - 1) * page) < row:
+            apart = base + min(max(p, 1 - a.shape[1]), b.shape[1] - 1) * page
+            if -other_row < apart < row:
                 return True
     return False
 

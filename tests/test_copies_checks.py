@@ -41,3 +41,26 @@ def test_parts_of_one_tensor():
         assert ops._meet(x, y) == want
         seen.add(want)
     assert seen == {True, False}
+
+
+def test_parts_of_one_tensor_with_rows_of_several_lengths_and_types():
+    """Keys longer than values, side by side in one row or shared by a byte: the places that each covers, one by one."""
+    whole = torch.zeros(4 * 6 * 20, dtype=torch.int32)
+    first = whole.data_ptr()
+
+    def part(dtype, row, at, pages=6, layers=4):
+        size = torch.empty((), dtype=dtype).element_size()
+        return whole.view(dtype).as_strided((layers, pages, 1, row), (6 * 80 // size, 80 // size, row, 1), at)
+
+    def places(t):
+        size = t.element_size()
+        return {t.data_ptr() - first + size * (l * t.stride(0) + p * t.stride(1) + i) + k for l in range(t.shape[0]) for p in range(t.shape[1])
+                for i in range(t.shape[3]) for k in range(size)}
+    parts = [part(torch.int32, 12, 0), part(torch.int32, 8, 12), part(torch.int32, 9, 11), part(torch.int16, 16, 24), part(torch.int16, 17, 23),
+             part(torch.int8, 32, 48), part(torch.int8, 33, 47), part(torch.int32, 20, 20, pages=5), part(torch.int32, 5, 60, pages=2, layers=3)]
+    seen = set()
+    for x, y in itertools.product(parts, parts):
+        want = bool(places(x) & places(y))
+        assert ops._meet(x, y) == want, (x.shape, y.shape)
+        seen.add(want)
+    assert seen == {True, False}
